@@ -8,7 +8,7 @@ MI355X-native underneath:
 
 - ``RcclCoreBackend``: our C++/HIP extension (``mgx_comm``) driving RCCL
   directly — one communicator per job, ncclAllReduce on a dedicated
-  high-priority non-blocking HIP stream, hipEvent-based handles so
+  non-blocking HIP stream, hipEvent-based handles so
   ``synchronize`` is a device-side stream-wait, not a host stall.
   Bootstrap: the ncclUniqueId is exchanged over a torch.distributed gloo
   group (env-var rendezvous, torchrun-compatible; no MPI anywhere).
@@ -164,7 +164,7 @@ class _RcclCoreHandle(Handle):
 class RcclCoreBackend:
     """Native RCCL comm core (C++ extension mgx_comm).
 
-    Dedicated non-blocking high-priority HIP stream for collectives,
+    Dedicated non-blocking HIP stream for collectives,
     hipEvent handles; the ncclUniqueId is exchanged through a gloo group.
     """
 

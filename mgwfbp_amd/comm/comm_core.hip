@@ -100,12 +100,11 @@ void init(int rank, int size, const std::string& uid_bytes) {
   ncclUniqueId id;
   memcpy(id.internal, uid_bytes.data(), NCCL_UNIQUE_ID_BYTES);
   CHECK_NCCL(ncclCommInitRank(&g_core.comm, size, id, rank));
-  // Dedicated non-blocking stream at the device's highest priority so
-  // collectives are scheduled ahead of bulk compute and overlap backward.
-  int least, greatest;
-  CHECK_HIP(hipDeviceGetStreamPriorityRange(&least, &greatest));
-  CHECK_HIP(hipStreamCreateWithPriority(&g_core.comm_stream,
-                                        hipStreamNonBlocking, greatest));
+  // Dedicated non-blocking stream, so that collectives overlap backward.
+  // It has the default priority like every other stream: work on streams
+  // of different priorities has hung on this hardware.
+  CHECK_HIP(hipStreamCreateWithFlags(&g_core.comm_stream,
+                                     hipStreamNonBlocking));
   g_core.rank = rank;
   g_core.size = size;
   g_core.initialized = true;
