@@ -125,14 +125,14 @@ def mgwfbp(dnn, dataset, data_dir, nworkers, lr, batch_size, nsteps_update,
                 _, hidden = trainer.train(1, hidden=hidden)
             if dnn in ('lstm', 'lstman4') and comm.size() <= 1:
                 # single-process: no hooks fire, so the optimizer's
-                # internal device-side per-group clip never runs — clip
-                # externally (reference dist_trainer.py:89-94). At
-                # world>1 norm_clip is honored inside synchronize()
-                # (device-side, no .item(); the reference factory
-                # dropped the arg — SURVEY.md §7.5).
-                torch.nn.utils.clip_grad_norm_(trainer.net.parameters(),
-                                               norm_clip)
-            trainer.update_model()
+                # internal device-side per-group clip never runs — the
+                # update itself clips by the global norm (reference
+                # dist_trainer.py:89-94 clips before it). At world>1
+                # norm_clip is honored inside synchronize() (device-side,
+                # no .item(); the reference factory dropped the arg).
+                trainer.update_model(max_grad_norm=norm_clip)
+            else:
+                trainer.update_model()
             optimizer.train_epoch = trainer.train_epoch
             times.append(time.time() - s)
         if i % display == 0 and i > 0 and rank == 0:

@@ -452,16 +452,34 @@ class _DistributedOptimizer(torch.optim.Optimizer):
         norm_clip = (1.0 / comm.size()) ** 0.5 * self._norm_clip
         _k.l2norm_clip_(flat, norm_clip)
 
-    def step(self, closure=None):
+    def step(self, closure=None, max_grad_norm=None):
+        """One update. ``max_grad_norm`` clips the gradients of all
+        parameters by their norm taken together: inside the fused update,
+        which then never writes clipped gradients, or in place before the
+        wrapped optimizer's loop. (``norm_clip`` of the factory is another
+        thing: it clips each merge group by itself after its all-reduce, as
+        the reference does.)"""
+        if max_grad_norm is not None:
+            if closure is not None:
+                raise ValueError('max_grad_norm needs gradients that are '
+                                 'there already: give no closure')
+            if not max_grad_norm >= 0.0:
+                raise ValueError('max_grad_norm must not be negative: %r'
+                                 % (max_grad_norm,))
         if not self.local and comm.size() > 1:
             self.synchronize()
         if self._fused_sgd is not None and closure is None:
             lr = self.param_groups[0]['lr']
             if all(g['lr'] == lr for g in self.param_groups):
-                self._fused_sgd.step(lr=lr)
+                self._fused_sgd.step(lr=lr, max_norm=max_grad_norm)
                 return None
             # per-group LRs diverged (user schedule): the single-launch
             # fused kernel carries one LR — use the torch loop instead
+        if max_grad_norm is not None:
+            from .kernels import grad_clip
+            grad_clip.clip_grad_norm_(
+                [p for g in self.param_groups for p in g['params']],
+                max_grad_norm)
         return super(self.__class__, self).step(closure)
 
     def zero_grad(self, set_to_none=False):

@@ -414,8 +414,13 @@ class DLTrainer:
     def zero_grad(self):
         self.optimizer.zero_grad()
 
-    def update_model(self):
-        self.optimizer.step()
+    def update_model(self, max_grad_norm=None):
+        """The optimizer's step; ``max_grad_norm`` clips the gradients by
+        their global norm (DistributedOptimizer only)."""
+        if max_grad_norm is None:
+            self.optimizer.step()
+        else:
+            self.optimizer.step(max_grad_norm=max_grad_norm)
 
     def update_optimizer(self, optimizer):
         self.optimizer = optimizer

@@ -1,6 +1,6 @@
 """Loaders and Python wrappers for the in-tree HIP extensions.
 
-Two extensions, built IN-TREE by ``setup.py build_ext --inplace`` (or
+The extensions of this module, built IN-TREE by ``setup.py build_ext --inplace`` (or
 ``__graft_entry__.build()``) so the .so files travel with the repo
 snapshot to GPU boxes:
 
@@ -115,11 +115,24 @@ class FusedSGD:
     def set_lr(self, lr):
         self._lr_buf.fill_(float(lr))
 
-    def step(self, lr, grad_scale=1.0):
+    def step(self, lr, grad_scale=1.0, max_norm=None, eps=1e-6):
+        """One update with the gradients times ``grad_scale``. With
+        ``max_norm`` they are also scaled so that their norm over all
+        tensors is at most that, as they are read: the gradients in memory
+        stay as they are. Returns that norm (before clipping), a float32
+        scalar on the device; None without ``max_norm``."""
+        if max_norm is not None and not (max_norm >= 0.0 and eps >= 0.0):
+            raise ValueError('max_norm and eps must not be negative: %r, %r'
+                             % (max_norm, eps))
         if self._lr_buf.numel() and \
                 not torch.cuda.is_current_stream_capturing():
             # buffer mode outside capture: keep the device LR current
             self._lr_buf.fill_(float(lr))
+        if max_norm is not None:
+            return self.ext.multi_tensor_sgd_clipped(
+                self._t_tensors, self._t_chunks, self._nchunks, float(lr),
+                self._lr_buf, self.momentum, self.dampening, self.nesterov,
+                float(grad_scale), float(max_norm), float(eps))
         self.ext.multi_tensor_sgd(self._t_tensors, self._t_chunks,
                                   self._nchunks, float(lr), self._lr_buf,
                                   self.momentum, self.dampening,

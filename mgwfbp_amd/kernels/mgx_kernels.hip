@@ -6,7 +6,8 @@
 // small per-tensor kernels at dl_trainer.py:244-248):
 //
 //   multi_tensor_sgd     — fused SGD + momentum + weight-decay (+nesterov)
-//                          over ALL parameters in ONE launch
+//                          over ALL parameters in ONE launch; with
+//                          global-norm clipping folded in, in two
 //   multi_tensor_pack    — gather per-layer grads into a flat comm buffer
 //                          with optional fp32->bf16/fp16 cast + scale
 //   multi_tensor_unpack  — scatter flat buffer back with cast + scale
@@ -66,13 +67,39 @@ struct Chunk {
 // lr_ptr: optional device-resident learning rate — lets a hipGraph
 // capture of the step keep a changing LR schedule without re-capture
 // (the host fills the buffer before each replay).
+//
+// CLIP: the gradients' global norm comes as partial sums of squares that
+// sgd_norm_partials_kernel left; every block adds them up in the same
+// order and folds min(1, max_norm / (norm + eps)) into grad_scale, so
+// clipping costs one read of the gradients and writes none of them. Block
+// 0 leaves the norm of the scaled gradients in norm_out.
+template <bool CLIP>
 __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
     const Chunk* __restrict__ chunks, int nchunks,
     const TensorTriple* __restrict__ tensors, float lr,
     const float* __restrict__ lr_ptr, float momentum,
-    float dampening, bool nesterov, float grad_scale) {
+    float dampening, bool nesterov, float grad_scale,
+    const double* __restrict__ partials, int npartials, double max_norm,
+    double eps, float* __restrict__ norm_out) {
   if (lr_ptr != nullptr) lr = *lr_ptr;
-  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+  if constexpr (CLIP) {
+    __shared__ double wave_sums[kBlock / 64];
+    double acc = 0.;
+    for (int i = threadIdx.x; i < npartials; i += kBlock) acc += partials[i];
+    for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+    if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    double s = 0.;
+    for (int w = 0; w < kBlock / 64; ++w) s += wave_sums[w];
+    const double norm = sqrt(s) * fabs((double)grad_scale);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+    const double f = max_norm / (norm + eps);
+    if (!(f >= 1.)) grad_scale = (float)(grad_scale * f);  // NaN stays one
+  }
+  for (int k = blockIdx.x; k < nchunks; k += gridDim.x) {
+    // CLIP goes from the last chunk back: what the norm's pass read last
+    // is still in the 256 MB cache
+    const int c = CLIP ? nchunks - 1 - k : k;
     const Chunk ck = chunks[c];
     const TensorTriple t = tensors[ck.tensor_idx];
     const long n = min(kChunk, t.numel - ck.start);
@@ -160,6 +187,57 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
       }
       p[i] -= lr * dp;
     }
+  }
+}
+
+// Sums of squares of the gradients, one for each block, in 64 bits: they
+// neither overflow nor lose the squares of small gradients, and cost
+// nothing beside the loads.
+__global__ __launch_bounds__(kBlock) void sgd_norm_partials_kernel(
+    const Chunk* __restrict__ chunks, int nchunks,
+    const TensorTriple* __restrict__ tensors,
+    double* __restrict__ partials) {
+  double a0 = 0., a1 = 0.;
+  const long step = (long)blockDim.x * 4L;
+  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+    const Chunk ck = chunks[c];
+    const TensorTriple t = tensors[ck.tensor_idx];
+    const long n = min(kChunk, t.numel - ck.start);
+    const float* __restrict__ g = t.g + ck.start;
+    const long nvec = n & ~3L;
+    long i = threadIdx.x * 4L;
+    for (; i + 3 * step < nvec; i += 4 * step) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        v[u] = *reinterpret_cast<const float4*>(g + i + u * step);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        a0 = fma((double)v[u].x, (double)v[u].x, a0);
+        a1 = fma((double)v[u].y, (double)v[u].y, a1);
+        a0 = fma((double)v[u].z, (double)v[u].z, a0);
+        a1 = fma((double)v[u].w, (double)v[u].w, a1);
+      }
+    }
+    for (; i < nvec; i += step) {
+      const float4 v = *reinterpret_cast<const float4*>(g + i);
+      a0 = fma((double)v.x, (double)v.x, a0);
+      a1 = fma((double)v.y, (double)v.y, a1);
+      a0 = fma((double)v.z, (double)v.z, a0);
+      a1 = fma((double)v.w, (double)v.w, a1);
+    }
+    for (long j = nvec + threadIdx.x; j < n; j += blockDim.x)
+      a0 = fma((double)g[j], (double)g[j], a0);
+  }
+  double acc = a0 + a1;
+  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+  __shared__ double wave_sums[kBlock / 64];
+  if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.;
+    for (int w = 0; w < kBlock / 64; ++w) s += wave_sums[w];
+    partials[blockIdx.x] = s;
   }
 }
 
@@ -429,15 +507,48 @@ void multi_tensor_sgd(torch::Tensor t_tensors, torch::Tensor t_chunks,
   const float* lr_ptr =
       lr_buf.defined() && lr_buf.numel() > 0
           ? lr_buf.data_ptr<float>() : nullptr;
-  hipLaunchKernelGGL(multi_tensor_sgd_kernel, dim3(grid_for(nchunks)),
+  hipLaunchKernelGGL(multi_tensor_sgd_kernel<false>, dim3(grid_for(nchunks)),
                      dim3(kBlock), 0, c10::hip::getCurrentHIPStream().stream(),
                      reinterpret_cast<const Chunk*>(t_chunks.data_ptr()),
                      (int)nchunks,
                      reinterpret_cast<const TensorTriple*>(
                          t_tensors.data_ptr()),
                      (float)lr, lr_ptr, (float)momentum, (float)dampening,
-                     nesterov, (float)grad_scale);
+                     nesterov, (float)grad_scale, (const double*)nullptr, 0,
+                     0., 0., (float*)nullptr);
   CHECK_HIP(hipGetLastError());
+}
+
+// The update with the gradients clipped by their global norm; returns the
+// norm, float32, on the device.
+torch::Tensor multi_tensor_sgd_clipped(
+    torch::Tensor t_tensors, torch::Tensor t_chunks, long nchunks, double lr,
+    torch::Tensor lr_buf, double momentum, double dampening, bool nesterov,
+    double grad_scale, double max_norm, double eps) {
+  c10::DeviceGuard guard(t_tensors.device());
+  auto stream = c10::hip::getCurrentHIPStream().stream();
+  const float* lr_ptr =
+      lr_buf.defined() && lr_buf.numel() > 0
+          ? lr_buf.data_ptr<float>() : nullptr;
+  const auto* chunks = reinterpret_cast<const Chunk*>(t_chunks.data_ptr());
+  const auto* tensors =
+      reinterpret_cast<const TensorTriple*>(t_tensors.data_ptr());
+  const auto opts = torch::TensorOptions().device(t_tensors.device());
+  const int nparts = std::max(1, std::min((int)nchunks, 1024));
+  auto partials = torch::empty({nparts}, opts.dtype(torch::kDouble));
+  auto norm = torch::empty({}, opts.dtype(torch::kFloat));
+  hipLaunchKernelGGL(sgd_norm_partials_kernel, dim3(nparts), dim3(kBlock), 0,
+                     stream, chunks, (int)nchunks, tensors,
+                     partials.data_ptr<double>());
+  CHECK_HIP(hipGetLastError());
+  hipLaunchKernelGGL(multi_tensor_sgd_kernel<true>,
+                     dim3(std::max(1, grid_for(nchunks))), dim3(kBlock), 0,
+                     stream, chunks, (int)nchunks, tensors, (float)lr, lr_ptr,
+                     (float)momentum, (float)dampening, nesterov,
+                     (float)grad_scale, partials.data_ptr<double>(), nparts,
+                     max_norm, eps, norm.data_ptr<float>());
+  CHECK_HIP(hipGetLastError());
+  return norm;
 }
 
 std::vector<torch::Tensor> build_pack_table(
@@ -586,6 +697,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("build_sgd_table", &build_sgd_table,
         "Build device-side chunk table for fused SGD");
   m.def("multi_tensor_sgd", &multi_tensor_sgd, "Fused multi-tensor SGD");
+  m.def("multi_tensor_sgd_clipped", &multi_tensor_sgd_clipped,
+        "Fused multi-tensor SGD with global-norm clipping");
   m.def("build_pack_table", &build_pack_table,
         "Build device-side chunk table for pack/unpack/norm");
   m.def("multi_tensor_pack", &multi_tensor_pack,

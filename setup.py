@@ -4,6 +4,8 @@ Usage:  PYTORCH_ROCM_ARCH=gfx950 python setup.py build_ext --inplace
 
 Builds:
   mgwfbp_amd/kernels/mgx_kernels_ext*.so   (fused SGD / pack / unpack / norm)
+  mgwfbp_amd/kernels/mgx_bn_ext*.so        (NHWC BatchNorm and max pooling)
+  mgwfbp_amd/kernels/mgx_lm_ext*.so        (language-model operators)
   mgwfbp_amd/comm/mgx_comm_ext*.so         (RCCL comm core)
 
 The .so files are git-ignored but travel with the gpurun snapshot, so a
@@ -39,6 +41,13 @@ ext_modules = [
     CUDAExtension(
         name='mgwfbp_amd.kernels.mgx_bn_ext',
         sources=['mgwfbp_amd/kernels/bn_kernels.hip'],
+        extra_compile_args=common_args,
+    ),
+    CUDAExtension(
+        name='mgwfbp_amd.kernels.mgx_lm_ext',
+        sources=['mgwfbp_amd/kernels/lm_ext.hip',
+                 'mgwfbp_amd/kernels/grad_clip_kernels.hip'],
+        depends=['mgwfbp_amd/kernels/lm_common.h'],
         extra_compile_args=common_args,
     ),
     CUDAExtension(

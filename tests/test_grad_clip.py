@@ -1,0 +1,108 @@
+"""Global-norm clipping on the CPU: the plain forms, the refusals, and the
+paths that call them."""
+import math
+
+import pytest
+import torch
+
+from mgwfbp_amd import kernels as K
+from mgwfbp_amd.kernels import grad_clip as gc
+
+
+def _params(shapes, types=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for i, s in enumerate(shapes):
+        t = types[i] if types else torch.float32
+        p = torch.nn.Parameter(torch.zeros(s, dtype=t))
+        p.grad = torch.randn(s, generator=g).to(t)
+        out.append(p)
+    return out
+
+
+@pytest.mark.parametrize('max_norm', [0.0, 0.25, 1e6])
+def test_in_place_matches_torch(max_norm):
+    shapes = [(7, 5), (33,), (2, 3, 4, 5)]
+    a, b = _params(shapes), _params(shapes)
+    norm = gc.clip_grad_norm_(a, max_norm)
+    ref = torch.nn.utils.clip_grad_norm_(b, max_norm)
+    # both round a norm and a product: a few half steps of float32
+    assert torch.allclose(norm, ref, rtol=4 * 2.0 ** -24, atol=0)
+    for p, q in zip(a, b):
+        assert torch.allclose(p.grad, q.grad, rtol=8 * 2.0 ** -24, atol=0)
+
+
+def test_new_tensors_leave_the_gradients():
+    grads = [p.grad for p in _params([(5,), (6, 7)])]
+    before = [g.clone() for g in grads]
+    new, norm = gc.clip_grads(grads, 0.5)
+    assert all(torch.equal(g, b) for g, b in zip(grads, before))
+    assert float(norm) == pytest.approx(float(gc.grad_norm(grads)))
+    assert float(gc.grad_norm(new)) == pytest.approx(0.5, rel=1e-5)
+
+
+def test_none_and_empty():
+    p = torch.nn.Parameter(torch.zeros(3))
+    assert float(gc.clip_grad_norm_([p], 1.0)) == 0.0
+    assert float(gc.clip_grad_norm_([], 1.0)) == 0.0
+    assert gc.clip_grads([], 1.0)[0] == []
+    assert float(gc.grad_norm([])) == 0.0
+    p.grad = torch.ones(3)
+    assert float(gc.clip_grad_norm_(p, 10.0)) == pytest.approx(math.sqrt(3))
+
+
+@pytest.mark.parametrize('call', [
+    lambda: gc.clip_grads([torch.ones(2)], -1.0),
+    lambda: gc.clip_grads([torch.ones(2)], float('nan')),
+    lambda: gc.clip_grads([torch.ones(2)], 1.0, eps=-1e-3),
+    lambda: gc.clip_grad_norm_(_params([(2,)]), -0.5),
+])
+def test_refuses_limits(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_native_entry_refuses_host_tensors():
+    ext = gc.load_lm()
+    with pytest.raises(ValueError):
+        ext.grad_norm([torch.ones(3)])
+    with pytest.raises(ValueError):
+        ext.clip_grads_([torch.ones(3)], 1.0, 0.0)
+    with pytest.raises(RuntimeError):
+        ext.grad_norm([])
+    with pytest.raises(TypeError):
+        ext.clip_grads([1.0], 1.0, 0.0)
+
+
+def test_optimizer_step_clips_on_the_cpu():
+    """DistributedOptimizer.step(max_grad_norm=) without the fused update
+    equals clipping first and stepping then."""
+    from mgwfbp_amd.distributed_optimizer import DistributedOptimizer
+
+    def build():
+        torch.manual_seed(3)
+        net = torch.nn.Sequential(torch.nn.Linear(6, 5),
+                                  torch.nn.Linear(5, 2))
+        opt = DistributedOptimizer(
+            torch.optim.SGD(net.parameters(), lr=0.5, momentum=0.9),
+            named_parameters=list(net.named_parameters()))
+        opt.zero_grad()
+        (net(torch.ones(4, 6)).square().sum() * 10).backward()
+        return net, opt
+
+    a, oa = build()
+    b, ob = build()
+    oa.step(max_grad_norm=0.1)
+    torch.nn.utils.clip_grad_norm_(b.parameters(), 0.1)
+    ob.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-7)
+    with pytest.raises(ValueError):
+        oa.step(max_grad_norm=-1.0)
+
+
+def test_single_process_entry_uses_the_clipped_step():
+    import inspect
+    from mgwfbp_amd import dist_trainer
+    assert 'max_grad_norm' in inspect.getsource(dist_trainer.mgwfbp)
+    assert K.FusedSGD.step.__doc__
