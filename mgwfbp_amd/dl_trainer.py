@@ -33,6 +33,7 @@ from torch.utils.data.distributed import DistributedSampler
 from . import models
 from . import settings
 from . import data as mgx_data
+from .kernels.token_loss import MgxCrossEntropyLoss, token_log_probs
 from .settings import logger
 
 # MIOpen autotune. Measured on MI355X (resnet50 bs128 bf16 NHWC):
@@ -190,6 +191,12 @@ class DLTrainer:
         if dataset == 'an4':
             self.criterion = nn.CTCLoss(blank=0, reduction='sum',
                                         zero_infinity=True)
+        elif dataset == 'ptb':
+            # a vocabulary of classes: one read of the logits (torch's own
+            # on the CPU)
+            self.criterion = (
+                MgxCrossEntropyLoss() if settings.USE_HIP_KERNELS
+                else nn.CrossEntropyLoss()).to(self.device)
         else:
             self.criterion = nn.CrossEntropyLoss().to(self.device)
 
@@ -230,6 +237,8 @@ class DLTrainer:
         self._loss_accum = None
         self.avg_loss_per_epoch = 0.0
         self.accuracy = 0.0
+        self.top5_accuracy = 0.0      # of the word-level model's test()
+        self.mean_entropy = 0.0
         self.loss = 0.0
         self.times = []
         self.display = 40
@@ -537,7 +546,7 @@ class DLTrainer:
     def test(self, epoch=0):
         self.net.eval()
         correct1 = correct5 = total = 0
-        total_loss = 0.0
+        total_loss = total_entropy = total_top5 = 0.0
         total_wer = 0.0
         nbatches = 0
         decoder = (models.GreedyDecoder() if self.dataset == 'an4'
@@ -566,10 +575,13 @@ class DLTrainer:
                     if x.size(0) != self.net.batch_size:
                         continue
                     out, _ = self.net(x, hidden)
-                    loss = self.criterion(
-                        out.contiguous().view(-1, self.net.ntokens),
-                        y.contiguous().view(-1))
-                    total_loss += loss.item()
+                    r = token_log_probs(out, y,
+                                        top_k=min(5, self.net.ntokens))
+                    # accumulated on the device, read back at the end
+                    total_loss -= r.log_probs.mean()
+                    total_entropy += r.entropy.mean()
+                    total_top5 += (r.top_ids == y.unsqueeze(-1)).any(
+                        -1).float().mean()
                     nbatches += 1
                     continue
                 x, y = batch
@@ -588,8 +600,12 @@ class DLTrainer:
             return wer
         if self.dnn == 'lstm':
             import math
-            ppl = math.exp(total_loss / max(nbatches, 1))
-            logger.info('epoch %d test perplexity: %.4f', epoch, ppl)
+            ppl = math.exp(float(total_loss) / max(nbatches, 1))
+            self.mean_entropy = float(total_entropy) / max(nbatches, 1)
+            self.top5_accuracy = float(total_top5) / max(nbatches, 1)
+            logger.info('epoch %d test perplexity: %.4f entropy %.4f top-5 '
+                        '%.4f', epoch, ppl, self.mean_entropy,
+                        self.top5_accuracy)
             return ppl
         acc1 = correct1 / max(total, 1)
         acc5 = correct5 / max(total, 1)

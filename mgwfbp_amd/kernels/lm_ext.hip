@@ -12,6 +12,13 @@ std::tuple<std::vector<torch::Tensor>, torch::Tensor> clip_grads(
 torch::Tensor clip_grads_(const std::vector<torch::Tensor>& grads,
                           double max_norm, double eps);
 
+torch::Tensor cross_entropy(const torch::Tensor& logits,
+                            const torch::Tensor& targets, int64_t ignore,
+                            int64_t reduction);
+std::vector<torch::Tensor> token_log_probs(const torch::Tensor& logits,
+                                           const torch::Tensor& targets,
+                                           int64_t k, int64_t ignore);
+
 }  // namespace mgx
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -20,4 +27,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "New gradients scaled to a global norm, and the norm");
   m.def("clip_grads_", &mgx::clip_grads_,
         "Scale gradients in place to a global norm; returns the norm");
+  m.def("cross_entropy", &mgx::cross_entropy,
+        "Cross entropy of logits and class indices (differentiable)");
+  m.def("token_log_probs", &mgx::token_log_probs,
+        "Log probabilities of given tokens, entropy, best alternatives");
 }

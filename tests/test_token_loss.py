@@ -1,0 +1,122 @@
+"""Cross entropy and token log probabilities on the CPU: the plain forms'
+formulas and gradients, and the refusals."""
+import math
+
+import pytest
+import torch
+
+from mgwfbp_amd.kernels import token_loss as tl
+from mgwfbp_amd.kernels.grad_clip import load_lm
+
+NEG = float('-inf')
+
+
+def test_formulas_in_64_bits():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(3, 4, 11, generator=g, dtype=torch.float64)
+    x[0, 0, 3:] = NEG
+    t = torch.randint(0, 3, (3, 4), generator=g)
+    r = tl.token_log_probs(x, t, top_k=4)
+    for i in range(3):
+        for j in range(4):
+            v = x[i, j].tolist()
+            s = math.fsum(math.exp(a) for a in v)
+            p = [math.exp(a) / s for a in v]
+            lp = math.log(p[int(t[i, j])])
+            h = -math.fsum(q * math.log(q) for q in p if q > 0)
+            order = sorted(range(11), key=lambda k: (-v[k], k))[:4]
+            assert float(r.log_probs[i, j]) == pytest.approx(lp, abs=1e-12)
+            assert float(r.entropy[i, j]) == pytest.approx(h, abs=1e-12)
+            assert r.top_ids[i, j].tolist() == order
+    ce = tl.cross_entropy(x, t, reduction='none')
+    assert torch.allclose(ce, -r.log_probs, atol=1e-12)
+    assert tl.cross_entropy(x, t).item() == pytest.approx(ce.mean().item())
+    assert tl.cross_entropy(x, t, reduction='sum').item() == \
+        pytest.approx(ce.sum().item())
+
+
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 7, generator=g, dtype=torch.float64,
+                    requires_grad=True)
+    t = torch.tensor([0, 6, -100, 3])
+    assert torch.autograd.gradcheck(
+        lambda a: tl.token_log_probs(a, t)[:2], (x,))
+    assert torch.autograd.gradcheck(
+        lambda a: tl.cross_entropy(a, t), (x,))
+
+
+def test_masked_classes_have_no_gradient():
+    x = torch.tensor([[0.5, NEG, -1.0, NEG]], requires_grad=True)
+    r = tl.token_log_probs(x, torch.tensor([2]))
+    (r.log_probs + r.entropy).sum().backward()
+    assert torch.isfinite(x.grad).all()
+    assert x.grad[0, 1] == 0 and x.grad[0, 3] == 0
+
+
+def test_ignored():
+    x = torch.randn(3, 5)
+    t = torch.tensor([-100, 2, -100])
+    assert tl.cross_entropy(x, t).item() == pytest.approx(
+        tl.cross_entropy(x[1:2], t[1:2]).item())
+    assert torch.isnan(tl.cross_entropy(x, torch.full((3,), -100)))
+    assert tl.token_log_probs(x, t).log_probs[0] == 0
+
+
+@pytest.mark.parametrize('error,call', [
+    (ValueError, lambda x, t: tl.cross_entropy(x, t, reduction='max')),
+    (ValueError, lambda x, t: tl.cross_entropy(x, t[:2])),
+    (TypeError, lambda x, t: tl.cross_entropy(x, t.float())),
+    (ValueError, lambda x, t: tl.token_log_probs(x, t, top_k=6)),
+    (ValueError, lambda x, t: tl.token_log_probs(x, t, top_k=-1)),
+    (ValueError, lambda x, t: tl.token_log_probs(x[:, :0], t)),
+    (IndexError, lambda x, t: tl.token_log_probs(x, t + 5)),
+    (IndexError, lambda x, t: tl.cross_entropy(x, t + 5)),
+])
+def test_refusals(error, call):
+    with pytest.raises(error):
+        call(torch.randn(3, 5), torch.tensor([0, 1, 2]))
+
+
+def test_native_entries_refuse_host_tensors():
+    ext = load_lm()
+    x, t = torch.randn(3, 5), torch.tensor([0, 1, 2])
+    with pytest.raises(ValueError):
+        ext.cross_entropy(x, t, -100, 1)
+    with pytest.raises(ValueError):
+        ext.token_log_probs(x, t, 0, -100)
+
+
+def test_module_is_torch_on_the_cpu():
+    x, t = torch.randn(6, 9), torch.randint(0, 9, (6,))
+    for kw in ({}, dict(reduction='sum'), dict(label_smoothing=0.1),
+               dict(weight=torch.rand(9))):
+        a = tl.MgxCrossEntropyLoss(**kw)(x, t)
+        b = torch.nn.CrossEntropyLoss(**kw)(x, t)
+        assert torch.equal(a, b)
+
+
+def test_word_level_evaluation():
+    """DLTrainer.test() scores the word-level model through
+    token_log_probs: the same perplexity as the mean cross entropy."""
+    from mgwfbp_amd.dl_trainer import DLTrainer
+    from mgwfbp_amd.models import lstm
+    torch.manual_seed(0)
+    t = DLTrainer(rank=0, size=1, dist=False, batch_size=4, ngpus=0,
+                  data_dir='', dataset='ptb', dnn='lstm', lr=1.0, nworkers=1,
+                  prefix='t', synthetic=True)
+    t.net = lstm(vocab_size=10000, batch_size=4, embedding_dim=8,
+                 hidden_dim=8)
+    t.testloader = [b for b, _ in zip(t.testloader, range(3))]
+    ppl = t.test(0)
+    t.net.eval()
+    total = 0.0
+    with torch.no_grad():
+        for x, y in t.testloader:
+            out, _ = t.net(x, t.net.init_hidden())
+            total += torch.nn.functional.cross_entropy(
+                out.view(-1, 10000), y.view(-1)).item()
+    assert ppl == pytest.approx(math.exp(total / 3), rel=1e-5)
+    assert 0.0 <= t.top5_accuracy <= 1.0
+    # nearly uniform over 10000 words
+    assert t.mean_entropy == pytest.approx(math.log(10000), rel=0.05)

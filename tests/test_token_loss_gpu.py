@@ -1,0 +1,464 @@
+"""Token loss kernels against 64-bit arithmetic on the same logits.
+
+Tolerances, with u = 2^-24 (half a step of float32). A term e^(x-m) is off by
+the rounding of x-m (u |x-m|), of its product with log2 e (u |x-m| log2 e, in
+the exponent, so times ln 2: u |x-m|) and of exp2 (2u): with |x-m| <= R on
+the terms that matter, (2R + 2) u relative. Rescaling to a new maximum
+repeats that for each of at most log-many rises and each merge; runs of n
+values in float32 add n u at the very worst and sqrt(n) u in practice, where
+n, a thread's share, is V / 256 or V / 1024. R: terms below e^-16 of the
+largest are under 2^-23 of the sum. So s is within
+S = (2 * 16 * 4 + V / 256 + 64) u of itself, relative: 192 u for small V,
+below 2^-16 throughout these tests (V <= 70001 gives 465 u = 2^-15.1, so
+REL = 2^-15 is used for s). log s is then off by REL at most, absolutely,
+plus u |log s|, and x_t - m by u |x_t - m|.
+"""
+import pytest
+import torch
+
+from mgwfbp_amd.kernels import token_loss as tl
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+REL = 2.0 ** -15
+NEG = float('-inf')
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# one class, less than a vector, around vectors and blocks, odd, split rows
+SIZES = [(1, 1), (3, 2), (5, 7), (2, 255), (3, 256), (4, 1023), (2, 4096),
+         (3, 4097), (700, 1000), (1, 10000), (20, 10001), (2, 50001),
+         (1, 70001), (600, 2049)]
+
+
+def _make(rows, vocab, kind, seed=0, scale=3.0):
+    g = torch.Generator().manual_seed(seed * 1000003 + rows * 131 + vocab)
+    x = (torch.randn(rows, vocab, generator=g) * scale).to(kind).cuda()
+    t = torch.randint(0, vocab, (rows,), generator=g).cuda()
+    return x, t
+
+
+def _exact(x):
+    x = x.detach().double()
+    # the maximum goes first: beside a row of lowest values log V would be
+    # lost in 64 bits too
+    x = x - x.amax(1, keepdim=True)
+    log = x - x.exp().sum(1, keepdim=True).log()
+    p = log.exp()
+    h = -(p * log.masked_fill(log == NEG, 0.0)).sum(1)
+    return log, p, h
+
+
+def _near_log(got, want, x):
+    """Log probabilities and entropies: REL, and u of what is subtracted."""
+    assert got.dtype == torch.float32
+    size = x.detach().double().masked_fill(x == NEG, 0.0).abs().amax()
+    far = REL + 4 * U * (2 * float(size) + 16)
+    off = (got.double() - want).abs()
+    worst = float(off.detach().max())
+    assert worst <= far, (worst, far)
+
+
+def _near_grad(got, want, p, coef, kind):
+    """A gradient's entry is p (a + b log p) + c: relative 2 REL of the
+    magnitudes that go in, and half a step of the type, or half its least
+    subnormal."""
+    assert got.dtype == kind
+    tiny = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126,
+            torch.float16: 2.0 ** -24}[kind]
+    far = torch.finfo(kind).eps / 2 * want.abs() + 2 * REL * coef * p + \
+        4 * U * coef + tiny
+    off = (got.double() - want).abs()
+    assert bool((off <= far).all()), float((off - far).max())
+
+
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('rows,vocab', SIZES)
+def test_log_probs_entropy_and_best(rows, vocab, kind):
+    x, t = _make(rows, vocab, kind)
+    log, p, h = _exact(x)
+    for k in {0, 1, min(5, vocab), min(64, vocab)}:
+        r = tl.token_log_probs(x, t, top_k=k)
+        _near_log(r.log_probs, log.gather(1, t[:, None])[:, 0], x)
+        _near_log(r.entropy, h, x)
+        ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
+        assert r.top_ids.dtype == torch.int64
+        assert torch.equal(r.top_ids, ids)
+        if k:
+            _near_log(r.top_log_probs, log.gather(1, ids), x)
+        assert r.top_log_probs.shape == (rows, k)
+
+
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('rows,vocab', SIZES)
+def test_log_probs_gradient(rows, vocab, kind):
+    x, t = _make(rows, vocab, kind, seed=1)
+    x.requires_grad_(True)
+    log, p, h = _exact(x)
+    g = torch.Generator().manual_seed(9)
+    gl = torch.randn(rows, generator=g).cuda()
+    ge = torch.randn(rows, generator=g).cuda()
+    for use_l, use_e in ((1, 1), (1, 0), (0, 1)):
+        r = tl.token_log_probs(x, t)
+        outs = [o for o, u in ((r.log_probs, use_l), (r.entropy, use_e))
+                if u]
+        got, = torch.autograd.grad(
+            outs, x, [g for g, u in ((gl, use_l), (ge, use_e)) if u])
+        a, b = gl.double()[:, None] * use_l, ge.double()[:, None] * use_e
+        want = -p * (a + b * (log + h[:, None]))
+        want[torch.arange(rows), t] += a[:, 0]
+        coef = a.abs() + b.abs() * (log.abs() + h[:, None].abs() + 1)
+        _near_grad(got, want, p, coef, kind)
+
+
+@pytest.mark.parametrize('wide', [torch.int64, torch.int32])
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('rows,vocab', SIZES)
+def test_cross_entropy(rows, vocab, kind, wide):
+    x, t = _make(rows, vocab, kind, seed=2)
+    x.requires_grad_(True)
+    log, p, _ = _exact(x)
+    t[::3] = -100
+    if rows == 1:
+        t[0] = vocab - 1
+    keep = t != -100
+    at = torch.where(keep, t, torch.zeros_like(t))
+    nll = torch.where(keep, -log.gather(1, at[:, None])[:, 0],
+                      torch.zeros((), dtype=torch.float64, device='cuda'))
+    n = int(keep.sum())
+    hot = torch.zeros_like(p)
+    hot[torch.arange(rows), at] = 1.0
+    t = t.to(wide)
+    each = tl.cross_entropy(x, t, reduction='none')
+    _near_log(each, nll, x)
+    assert bool((each[~keep] == 0).all())
+    w = torch.rand(rows, generator=torch.Generator().manual_seed(3)).cuda()
+    for red, coef in (('none', w.double()), ('sum', torch.ones_like(nll)),
+                      ('mean', torch.full_like(nll, 1.0 / max(n, 1)))):
+        loss = tl.cross_entropy(x, t, reduction=red)
+        if red == 'none':
+            got, = torch.autograd.grad(loss, x, w)
+        else:
+            want = nll.sum() / (n if red == 'mean' else 1)
+            if n:
+                _near_log(loss / (1 if red == 'mean' else n),
+                          want / (1 if red == 'mean' else n), x)
+            got, = torch.autograd.grad(loss, x)
+        if n == 0 and red == 'mean':
+            assert torch.isnan(loss)
+        c = (coef * keep)[:, None]
+        _near_grad(got, (p - hot) * c, p, c, kind)
+        assert bool((got[~keep] == 0).all())
+
+
+@pytest.mark.parametrize('scale', [0.25, 3.0, 65536.0])
+@pytest.mark.parametrize('kind', TYPES)
+def test_loss_scaled_afterwards(kind, scale):
+    """The gradient that comes in is not one: it is rounded once all the
+    same."""
+    x, t = _make(37, 1003, kind, seed=4)
+    x.requires_grad_(True)
+    log, p, _ = _exact(x)
+    hot = torch.zeros_like(p)
+    hot[torch.arange(37), t] = 1.0
+    got, = torch.autograd.grad(tl.cross_entropy(x, t) * scale, x)
+    _near_grad(got, (p - hot) * scale / 37, p,
+               torch.full_like(p, scale / 37), kind)
+
+
+def test_backward_twice_and_after():
+    x, t = _make(33, 515, torch.float32, seed=5)
+    x.requires_grad_(True)
+    loss = tl.cross_entropy(x, t)
+    a, = torch.autograd.grad(loss, x, retain_graph=True)
+    b, = torch.autograd.grad(loss, x, torch.tensor(2.0, device='cuda'),
+                             retain_graph=True)
+    c, = torch.autograd.grad(loss, x, retain_graph=True)
+    keep = a.clone()
+    a.mul_(7.0)                          # the caller's own by now
+    d, = torch.autograd.grad(loss, x)
+    assert torch.allclose(b, 2 * keep, rtol=4 * U, atol=0)
+    assert torch.allclose(c, keep, rtol=4 * U, atol=0)
+    assert torch.allclose(d, keep, rtol=4 * U, atol=0)
+    loss = tl.cross_entropy(x, t)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, x, create_graph=True)
+
+
+def test_logits_changed_before_the_backward():
+    x, t = _make(8, 100, torch.float32, seed=6)
+    w = torch.ones((), device='cuda', requires_grad=True)
+    y = x * w
+    loss = tl.cross_entropy(y, t)
+    y.detach().add_(1.0)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_gradient_against_differences():
+    """One entry at a time, by the plain formula in 64 bits on either
+    side."""
+    x, t = _make(2, 6, torch.float32, seed=7)
+    x.requires_grad_(True)
+    r = tl.token_log_probs(x, t)
+    got, = torch.autograd.grad((r.log_probs * 2 + r.entropy).sum(), x)
+    step = 1e-4
+    for i in range(2):
+        for j in range(6):
+            v = []
+            for s in (step, -step):
+                y = x.detach().double().clone()
+                y[i, j] += s
+                log, _, h = _exact(y)
+                v.append(float(2 * log[torch.arange(2), t].sum() + h.sum()))
+            # third derivatives are below 10, REL is what the kernel may lose
+            assert abs((v[0] - v[1]) / (2 * step) - float(got[i, j])) < \
+                4 * REL + 10 * step * step
+
+
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('vocab', [9, 1000, 40001])
+def test_masks(vocab, kind):
+    """-inf, the type's lowest value, and rows with nothing left."""
+    low = torch.finfo(kind).min
+    x, t = _make(6, vocab, kind, seed=8)
+    x[0, 3:] = NEG                       # three classes left
+    x[1, : vocab - 1] = NEG              # one, the last
+    x[2] = low                           # nothing but the lowest value
+    x[3, 1:] = low
+    x[4] = NEG                           # nothing at all
+    t[:] = torch.tensor([1, vocab - 1, 5, 0, 2, 4])
+    k = min(5, vocab)
+    x.requires_grad_(True)
+    r = tl.token_log_probs(x, t, top_k=k)
+    keep = [0, 1, 2, 3, 5]
+    y = x.detach().double()
+    # in the rows that differ from a constant by one value, float32 and
+    # 64 bits agree that e^(low - x) is 0
+    log, p, h = _exact(y)
+    for i in keep:
+        assert abs(float(r.log_probs[i].detach()) - float(log[i, t[i]])) < 2 * REL
+        assert abs(float(r.entropy[i].detach()) - float(h[i])) < 4 * REL
+    ids = torch.sort(x.detach(), dim=1, descending=True, stable=True)[1]
+    assert torch.equal(r.top_ids, ids[:, :k])
+    assert torch.isnan(r.log_probs[4]) and torch.isnan(r.entropy[4])
+    assert r.top_log_probs[0, 3:].tolist() == [NEG] * (k - 3)
+    got, = torch.autograd.grad((r.log_probs + r.entropy)[keep].sum(), x)
+    assert torch.isfinite(got[keep]).all()
+    assert bool((got[0, 3:] == 0).all()) and bool((got[1] == 0).all())
+    loss = tl.cross_entropy(x, t, reduction='none')
+    got, = torch.autograd.grad(loss[keep].sum(), x)
+    assert torch.isfinite(got[keep]).all()
+    # the empty row is no fault of its neighbours, and may be ignored
+    t[4] = -100
+    loss = tl.cross_entropy(x, t)
+    assert torch.isfinite(loss)
+    got, = torch.autograd.grad(loss, x)
+    assert torch.isfinite(got).all() and bool((got[4] == 0).all())
+
+
+@pytest.mark.parametrize('value', [float('nan'), float('inf')])
+def test_rows_that_are_not_finite(value):
+    x, t = _make(3, 5000, torch.float32, seed=9)
+    x[1, 4321] = value
+    r = tl.token_log_probs(x, t, top_k=3)
+    ref = torch.log_softmax(x, 1)[torch.arange(3), t]
+    assert torch.equal(torch.isnan(r.log_probs), torch.isnan(ref))
+    assert torch.isnan(r.entropy).tolist() == [False, True, False]
+    assert int(r.top_ids[1, 0]) == 4321
+    x.requires_grad_(True)
+    got, = torch.autograd.grad(
+        tl.cross_entropy(x, t, reduction='none').sum(), x)
+    assert torch.isnan(got[1]).all()
+    assert torch.isfinite(got[0]).all() and torch.isfinite(got[2]).all()
+
+
+@pytest.mark.parametrize('vocab', [64, 600, 5000, 60001])
+@pytest.mark.parametrize('k', [1, 20, 64])
+def test_equal_values(vocab, k):
+    """Ties, more of them than the search holds: the lowest index first."""
+    x = torch.zeros(3, vocab, device='cuda')
+    x[1, ::2] = -0.0                     # both zeros are the same value
+    x[2] = (torch.arange(vocab, device='cuda') % 3).float()
+    r = tl.token_log_probs(x, torch.zeros(3, dtype=torch.long,
+                                          device='cuda'), top_k=k)
+    ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(r.top_ids, ids)
+    assert torch.isfinite(r.top_log_probs).all()
+
+
+def test_targets_outside_the_classes():
+    """Nothing is read for them; they are NaN, and their neighbours are
+    not."""
+    x, t = _make(5, 300, torch.float32, seed=10)
+    t[1], t[3] = 300, -7
+    x.requires_grad_(True)
+    r = tl.token_log_probs(x, t)
+    assert torch.isnan(r.log_probs).tolist() == [False, True, False, True,
+                                                 False]
+    assert torch.isfinite(r.entropy).all()
+    each = tl.cross_entropy(x, t, reduction='none')
+    assert torch.isnan(each).tolist() == [False, True, False, True, False]
+    got, = torch.autograd.grad(each.sum(), x)
+    assert torch.isnan(got[1]).all() and torch.isfinite(got[0]).all()
+    loss = tl.cross_entropy(x, t)
+    assert torch.isnan(loss)
+    got, = torch.autograd.grad(loss, x)
+    assert torch.isnan(got[3]).all() and torch.isfinite(got[4]).all()
+
+
+@pytest.mark.parametrize('kind', TYPES)
+def test_strides_shapes_and_neighbours(kind):
+    big, _ = _make(12, 777, kind, seed=11)
+    t = torch.randint(0, 500, (2, 3), device='cuda')
+    for x in (big[:6, 5:705].reshape(2, 3, 700),
+              big.view(2, 6, 777)[:, ::2, 3:603],
+              big.t()[:600].t()[:6].view(2, 3, 600),
+              big[:1, :600].expand(6, 600).reshape(2, 3, 600),
+              big[:1, :600].expand(2, 3, 600)):
+        y = x.detach().clone().contiguous().view(6, -1)
+        a = tl.token_log_probs(x, t, top_k=3)
+        b = tl.token_log_probs(y, t.view(-1), top_k=3)
+        for u, v in zip(a, b):
+            assert torch.equal(u.reshape(v.shape), v)
+        z = x.detach().requires_grad_(True)
+        w = y.detach().requires_grad_(True)
+        gz, = torch.autograd.grad(tl.cross_entropy(z, t), z)
+        gw, = torch.autograd.grad(tl.cross_entropy(w, t.view(-1)), w)
+        assert gz.shape == x.shape
+        assert torch.allclose(gz.float().reshape(6, -1), gw.float(),
+                              rtol=torch.finfo(kind).eps, atol=0)
+
+
+def test_one_row_and_none():
+    x, _ = _make(1, 50, torch.float32)
+    v = x[0]
+    t = torch.tensor(3, device='cuda')
+    r = tl.token_log_probs(v, t, top_k=2)
+    assert r.log_probs.shape == () and r.top_ids.shape == (2,)
+    assert tl.cross_entropy(v, t, reduction='none').shape == ()
+    e = torch.zeros(0, 50, device='cuda', requires_grad=True)
+    none = torch.zeros(0, dtype=torch.long, device='cuda')
+    assert torch.isnan(tl.cross_entropy(e, none))
+    assert tl.cross_entropy(e, none, reduction='sum') == 0
+    assert tl.cross_entropy(e, none, reduction='none').shape == (0,)
+    assert tl.token_log_probs(e, none, top_k=2).top_ids.shape == (0, 2)
+    g, = torch.autograd.grad(tl.cross_entropy(e, none, reduction='sum'), e)
+    assert g.shape == (0, 50)
+
+
+def test_expanded_gradient_and_other_type():
+    x, t = _make(9, 400, torch.float32, seed=12)
+    x.requires_grad_(True)
+    a, = torch.autograd.grad(
+        tl.cross_entropy(x, t, reduction='none').sum(), x)
+    b, = torch.autograd.grad(tl.cross_entropy(x, t, reduction='sum'), x)
+    assert torch.allclose(a, b, rtol=8 * U, atol=0)
+    r = tl.token_log_probs(x, t)
+    c, = torch.autograd.grad(r.log_probs.double().sum(), x)
+    assert torch.allclose(c, -b, rtol=8 * U, atol=0)
+
+
+def test_far_rows():
+    """Row offsets past 2^31 elements."""
+    rows, vocab = 40000, 60000
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device='cuda')
+    x[-1], _ = _make(1, vocab, torch.bfloat16, seed=13)
+    t = torch.zeros(rows, dtype=torch.long, device='cuda')
+    t[-1] = vocab - 3
+    t[1:-1] = -100
+    last = x[-1:].clone().requires_grad_(True)
+    x.requires_grad_(True)
+    loss = tl.cross_entropy(x, t, reduction='sum')
+    g, = torch.autograd.grad(loss, x)
+    l2 = tl.cross_entropy(last, t[-1:], reduction='sum')
+    g2, = torch.autograd.grad(l2, last)
+    assert torch.allclose(g[-1:].float(), g2.float(),
+                          rtol=torch.finfo(torch.bfloat16).eps, atol=0)
+    assert bool((g[5] == 0).all()) and bool((g[rows - 2] == 0).all())
+    assert tl.token_log_probs(x.detach()[-2:], t[-2:],
+                              top_k=1).top_ids[1, 0] == x[-1].argmax()
+
+
+def test_refusals():
+    x, t = _make(4, 30, torch.float32)
+    for bad, error in ((dict(top_k=65), ValueError),
+                       (dict(top_k=31), ValueError),
+                       (dict(top_k=-1), ValueError)):
+        with pytest.raises(error):
+            tl.token_log_probs(x, t, **bad)
+    with pytest.raises(TypeError):
+        tl.cross_entropy(x.double(), t)
+    with pytest.raises(TypeError):
+        tl.cross_entropy(x, t.float())
+    with pytest.raises(ValueError):
+        tl.cross_entropy(x, t.cpu())
+    with pytest.raises(ValueError):
+        tl.cross_entropy(x, t[:3])
+    with pytest.raises(ValueError):
+        tl.cross_entropy(x, t, reduction='max')
+    with pytest.raises(ValueError):
+        tl.cross_entropy(x[:, :0], t)
+
+
+def test_module():
+    x, t = _make(40, 333, torch.float32, seed=14)
+    t[:4] = -100
+    for kw in ({}, dict(reduction='sum'), dict(reduction='none'),
+               dict(ignore_index=7), dict(label_smoothing=0.1),
+               dict(weight=torch.rand(333, device='cuda'))):
+        if kw.get('ignore_index') == 7:
+            t = t.clamp(min=0)
+        a, b = (x.clone().requires_grad_(True) for _ in range(2))
+        u = tl.MgxCrossEntropyLoss(**kw)(a, t)
+        v = torch.nn.CrossEntropyLoss(**kw)(b, t)
+        assert torch.allclose(u, v, rtol=1e-5, atol=1e-5)
+        u.sum().backward()
+        v.sum().backward()
+        assert torch.allclose(a.grad, b.grad, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize('rows,vocab', [(2, 50001), (300, 1001)])
+def test_captured(rows, vocab):
+    """Forward and backward in one graph, replayed between eager calls."""
+    x, t = _make(rows, vocab, torch.bfloat16, seed=15)
+    x.requires_grad_(True)
+
+    def call():
+        r = tl.token_log_probs(x, t, top_k=4)
+        g1, = torch.autograd.grad([r.log_probs, r.entropy], x,
+                                  [torch.ones_like(r.log_probs)] * 2)
+        loss = tl.cross_entropy(x, t)
+        g2, = torch.autograd.grad(loss * 3, x)
+        g3, = torch.autograd.grad(tl.cross_entropy(x, t), x)
+        return [r.log_probs, r.entropy, r.top_ids, g1, loss, g2, g3]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for k in range(4):
+        y, u = _make(rows, vocab, torch.bfloat16, seed=20 + k)
+        with torch.no_grad():
+            x.copy_(y)
+        t.copy_(u)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, call()):
+            assert torch.equal(a, b)
+
+
+def test_same_bits_every_time():
+    x, t = _make(64, 5003, torch.float32, seed=16)
+    x.requires_grad_(True)
+    first = None
+    for _ in range(3):
+        loss = tl.cross_entropy(x, t)
+        g, = torch.autograd.grad(loss, x)
+        if first is None:
+            first = (loss, g)
+        assert torch.equal(loss, first[0]) and torch.equal(g, first[1])
