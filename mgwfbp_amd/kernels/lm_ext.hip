@@ -12,6 +12,9 @@ std::tuple<std::vector<torch::Tensor>, torch::Tensor> clip_grads(
 torch::Tensor clip_grads_(const std::vector<torch::Tensor>& grads,
                           double max_norm, double eps);
 
+torch::Tensor embedding(const torch::Tensor& tokens,
+                        const torch::Tensor& weight, double scale,
+                        int64_t padding);
 torch::Tensor cross_entropy(const torch::Tensor& logits,
                             const torch::Tensor& targets, int64_t ignore,
                             int64_t reduction);
@@ -27,6 +30,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "New gradients scaled to a global norm, and the norm");
   m.def("clip_grads_", &mgx::clip_grads_,
         "Scale gradients in place to a global norm; returns the norm");
+  m.def("embedding", &mgx::embedding,
+        "Rows of a table by token, scaled (differentiable)");
   m.def("cross_entropy", &mgx::cross_entropy,
         "Cross entropy of logits and class indices (differentiable)");
   m.def("token_log_probs", &mgx::token_log_probs,

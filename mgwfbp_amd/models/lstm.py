@@ -6,6 +6,8 @@
 import torch
 import torch.nn as nn
 
+from ..kernels.embedding import MgxEmbedding
+
 
 class lstm(nn.Module):
     def __init__(self, vocab_size=10000, embedding_dim=1500, hidden_dim=1500,
@@ -17,7 +19,7 @@ class lstm(nn.Module):
         self.num_steps = num_steps
         self.batch_size = batch_size
         self.drop = nn.Dropout(dropout)
-        self.embedding = nn.Embedding(vocab_size, embedding_dim)
+        self.embedding = MgxEmbedding(vocab_size, embedding_dim)
         self.rnn = nn.LSTM(embedding_dim, hidden_dim, num_layers,
                            dropout=dropout, batch_first=True)
         self.fc = nn.Linear(hidden_dim, vocab_size)

@@ -46,6 +46,7 @@ ext_modules = [
     CUDAExtension(
         name='mgwfbp_amd.kernels.mgx_lm_ext',
         sources=['mgwfbp_amd/kernels/lm_ext.hip',
+                 'mgwfbp_amd/kernels/embedding_kernels.hip',
                  'mgwfbp_amd/kernels/grad_clip_kernels.hip',
                  'mgwfbp_amd/kernels/token_loss_kernels.hip'],
         depends=['mgwfbp_amd/kernels/lm_common.h'],
