@@ -10,6 +10,8 @@
 // tokens are sorted first, stably, and each run of one token is added up
 // in the order of its positions, in 32 bits, and rounded once.
 //
+// Up to 1024 tokens, owned_rows_kernel does all of it in one launch. More:
+//
 //   1. sort. Up to 16384 tokens one block sorts them in LDS (a stable
 //      radix sort, at most 8 bits a pass), while the launch's other blocks
 //      clear dW, which takes longer: the sort costs nothing then. More
@@ -43,16 +45,13 @@ __device__ __forceinline__ long token_at(const void* p, bool wide, long i) {
 
 // The first `cols` elements of a vector; the rest is zero.
 template <typename T>
-__device__ __forceinline__ void load_cols(const T* p, int cols, float* f) {
+__device__ __forceinline__ u32x4 load_cols(const T* p, int cols) {
   constexpr int V = Elem<T>::kVec;
-  if (cols >= V) {
-    const u32x4 v = load16(p);
+  if (cols >= V) return load16(p);
+  float f[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = Elem<T>::get(v, j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = j < cols ? Elem<T>::up(p[j]) : 0.f;
-  }
+  for (int j = 0; j < V; ++j) f[j] = j < cols ? Elem<T>::up(p[j]) : 0.f;
+  return Elem<T>::pack(f);
 }
 template <typename T>
 __device__ __forceinline__ void store_cols(T* p, int cols, const float* f) {
@@ -78,7 +77,7 @@ __global__ __launch_bounds__(kThreads) void gather_rows_kernel(
   const long first = (long)blockIdx.x * (kThreads * U);
   const long row0 = first / vecs;
   const unsigned off0 = (unsigned)(first - row0 * vecs);
-  float f[U][V];
+  u32x4 f[U];
   long row[U];
   int col[U];
 #pragma unroll
@@ -89,19 +88,22 @@ __global__ __launch_bounds__(kThreads) void gather_rows_kernel(
     if (row[u] < n) {
       const long t = token_at(tokens, wide, row[u]);
       if (t >= 0 && t < vocab) {
-        load_cols(weight + t * row_stride + col[u], dim - col[u], f[u]);
+        f[u] = load_cols(weight + t * row_stride + col[u], dim - col[u]);
       } else {
+        float nan[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[u][j] = __builtin_nanf("");
+        for (int j = 0; j < V; ++j) nan[j] = __builtin_nanf("");
+        f[u] = Elem<T>::pack(nan);
       }
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (row[u] < n) {
+      float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[u][j] *= scale;
-      store_cols(out + row[u] * dim + col[u], dim - col[u], f[u]);
+      for (int j = 0; j < V; ++j) y[j] = Elem<T>::get(f[u], j) * scale;
+      store_cols(out + row[u] * dim + col[u], dim - col[u], y);
     }
 }
 
@@ -354,6 +356,135 @@ __global__ __launch_bounds__(kThreads) void tile_scatter_kernel(
 }
 
 // ---------------------------------------------------------------- sums ---
+// Few tokens: one launch, no sort. A block owns kOwned rows of dW, far
+// apart (frequent tokens are often neighbours), and 64 vectors of columns;
+// it looks through all the tokens for those rows, keeping the order of
+// their positions, and writes each row's sum, or zeros. Each wave takes the
+// rows that are its own; a row with many tokens is taken by the whole
+// block, a quarter of the positions in each wave.
+constexpr int kOwned = 16;
+constexpr int kOwnedTokens = 1024;
+constexpr int kMany = 16;
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void owned_rows_kernel(
+    const void* __restrict__ tokens, bool wide, int n, long vocab,
+    long padding, int dim, int slices, float scale,
+    const T* __restrict__ dout, long row_stride, T* __restrict__ grad) {
+  constexpr int V = Elem<T>::kVec;
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kEach = kOwnedTokens / kWaves / 64;  // of a lane
+  __shared__ uint16_t found[kWaves][kOwnedTokens / kWaves];
+  __shared__ int length[kWaves];
+  __shared__ int count[kOwned];
+  __shared__ float part[kWaves][64][V];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned stride = (unsigned)((vocab + kOwned - 1) / kOwned);
+  const unsigned row0 = blockIdx.x / slices;     // and row0 + stride, ...
+  const int rows = (int)((vocab - row0 + stride - 1) / stride);
+  const int col = ((int)(blockIdx.x % slices) * 64 + lane) * V;
+  const int cols = dim - col;            // may be none
+  if (threadIdx.x < kOwned) count[threadIdx.x] = 0;
+  __syncthreads();
+
+  const int quarter = (n + kThreads - 1) / kThreads * 64;
+  const unsigned long long below = (1ull << lane) - 1;
+  long token[kEach];
+#pragma unroll
+  for (int g = 0; g < kEach; ++g) {
+    const int i = wave * quarter + g * 64 + lane;
+    token[g] = g * 64 < quarter && i < n ? token_at(tokens, wide, i) : -1;
+  }
+  int mine = 0;
+#pragma unroll
+  for (int g = 0; g < kEach; ++g) {
+    const unsigned t = (unsigned)token[g];
+    const unsigned r = t / stride;
+    const bool hit = token[g] >= 0 && token[g] < vocab &&
+        token[g] != padding && t - r * stride == row0;
+    const unsigned long long hits = __ballot(hit);
+    if (hit) {
+      const int i = wave * quarter + g * 64 + lane;
+      found[wave][mine + __popcll(hits & below)] = (uint16_t)(i << 4 | r);
+      atomicAdd(&count[r], 1);
+    }
+    mine += __popcll(hits);
+  }
+  if (lane == 0) length[wave] = mine;
+  __syncthreads();
+
+  float acc[V];
+  // adds a wave's finds for row r, in order
+  const auto add = [&](int w, int r) {
+    const int len = length[w];
+    for (int from = 0; from < len; from += 64) {
+      const int f = from + lane < len ? found[w][from + lane] : 0xffffffff;
+      unsigned long long left = __ballot(f >= 0 && (f & (kOwned - 1)) == r);
+      while (left) {
+        u32x4 v[8];
+        int have = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (left) {
+            const int at = __ffsll(left) - 1;
+            left &= left - 1;
+            const int pos = __builtin_amdgcn_readlane(f, at) >> 4;
+            if (cols > 0)
+              v[u] = load_cols(dout + pos * row_stride + col, cols);
+            have = u + 1;
+          }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (u < have) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] += Elem<T>::get(v[u], j);
+          }
+      }
+    }
+  };
+  const auto write = [&](int r) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] *= scale;
+    if (cols > 0)
+      store_cols(grad + (row0 + (long)r * stride) * dim + col, cols, acc);
+  };
+  const int counts = lane < rows ? count[lane] : 0;
+  const unsigned some = (unsigned)__ballot(counts > 0);
+  unsigned many = (unsigned)__ballot(counts > kMany);
+  // the rows without a token first: nothing waits for their stores
+  for (int r = wave; r < rows; r += kWaves)
+    if (!(some >> r & 1)) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = 0.f;
+      write(r);
+    }
+  for (int r = wave; r < rows; r += kWaves)
+    if ((some & ~many) >> r & 1) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = 0.f;
+      for (int w = 0; w < kWaves; ++w) add(w, r);
+      write(r);
+    }
+  for (; many; many &= many - 1) {
+    const int r = __ffs(many) - 1;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+    add(wave, r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[wave][lane][j] = acc[j];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w)
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += part[w][lane][j];
+      write(r);
+    }
+    __syncthreads();
+  }
+}
+
 struct Runs {
   const uint32_t* keys;
   const uint32_t* positions;
@@ -412,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void sum_runs_kernel(
   constexpr int U = 8;
   bool first = true;                     // the run at hand is the chunk's first
   for (int j0 = 0; j0 < n; j0 += U) {
-    float f[U][V];
+    u32x4 f[U];
     uint32_t ks[U + 1];
 #pragma unroll
     for (int u = 0; u <= U; ++u)
@@ -423,13 +554,13 @@ __global__ __launch_bounds__(kThreads) void sum_runs_kernel(
     for (int u = 0; u < U; ++u)
       if (j0 + u < n && cols > 0) {
         const uint32_t p = __builtin_amdgcn_readlane(pos, min(j0 + u, 63));
-        load_cols(dout + (long)p * row_stride + col, cols, f[u]);
+        f[u] = load_cols(dout + (long)p * row_stride + col, cols);
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (j0 + u < n && ks[u] < r.vocab) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += f[u][j];
+        for (int j = 0; j < V; ++j) acc[j] += Elem<T>::get(f[u], j);
         const bool end = j0 + u == n - 1;
         if (end || ks[u + 1] != ks[u]) {
           leave(ks[u], first && from > 0 && last_key == ks[u],
@@ -601,6 +732,25 @@ torch::Tensor weight_grad(const torch::Tensor& tokens,
   auto grad = torch::empty({vocab, dim}, dout.options());
   if (grad.numel() == 0) return grad;
   if (n == 0) return grad.zero_();
+  // Without a sort while the tokens are few and their rows mostly have one
+  // or none: each block then looks through all of them.
+  if (n <= kOwnedTokens && n <= 2 * vocab) {
+    with_elem(dout.scalar_type(), "the embedding gradient", [&](auto z) {
+      using T = decltype(z);
+      const long slices = ceil_div(dim, 64L * Elem<T>::kVec);
+      const long blocks = ceil_div(vocab, kOwned) * slices;
+      TORCH_CHECK_VALUE(blocks < (1L << 31), "the table is too large");
+      hipLaunchKernelGGL(owned_rows_kernel<T>, dim3(blocks), dim3(kThreads),
+                         0, current_stream(), tokens.data_ptr(),
+                         is_wide(tokens), (int)n, vocab, padding, (int)dim,
+                         (int)slices, scale,
+                         static_cast<const T*>(dout.data_ptr()),
+                         (long)dout.stride(0),
+                         static_cast<T*>(grad.data_ptr()));
+      CHECK_HIP(hipGetLastError());
+    });
+    return grad;
+  }
   const auto ints = tokens.options().dtype(torch::kInt);
   auto keys = torch::empty({n}, ints);
   auto positions = torch::empty({n}, ints);

@@ -62,7 +62,8 @@ def grad_norm(grads):
 @torch.no_grad()
 def clip_grads(grads, max_norm, eps=1e-6):
     """``(clipped, norm)``: new tensors, of the gradients' types, that hold
-    ``grads`` times ``min(1, max_norm / (norm + eps))``."""
+    ``grads`` times ``min(1, max_norm / (norm + eps))``. On a GPU they lie
+    in one new buffer, which lives as long as any of them."""
     grads = list(grads)
     max_norm, eps = _limits(max_norm, eps)
     if not grads:

@@ -26,7 +26,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 120;       // their addresses fit 4 KB of arguments
 constexpr int kChunk = 16384;          // elements of one block's turn
-constexpr int kMaxBlocks = 1024;       // 4 blocks of 4 waves on each CU
+constexpr int kMaxBlocks = 1024;       // that leave a partial sum
+constexpr int kMaxScaleBlocks = 2048;  // 8 blocks of 4 waves on each CU
 
 struct TensorList {
   const void* src[kMaxTensors];
@@ -49,7 +50,22 @@ __device__ __forceinline__ int tensor_of(const TensorList& l, int chunk) {
   return lo;
 }
 
-template <typename T>
+// Together larger than this, the gradients go past the 256 MB cache both
+// times; below, the second pass finds them there. Three passes over 64 and
+// 256 MB of gradients that were not there before: 36 and 159 us through the
+// cache, 40 and 137 us past it.
+constexpr long kPastBytes = 128L << 20;
+
+template <bool PAST>
+__device__ __forceinline__ u32x4 load_(const void* p) {
+  return PAST ? load16_past(p) : load16(p);
+}
+template <bool PAST>
+__device__ __forceinline__ void store_(void* p, u32x4 v) {
+  if (PAST) store16_past(p, v); else store16(p, v);
+}
+
+template <bool PAST, typename T>
 __device__ __forceinline__ double squares(const T* __restrict__ p, int n) {
   constexpr int V = Elem<T>::kVec;
   constexpr int kStep = kThreads * V;
@@ -59,7 +75,7 @@ __device__ __forceinline__ double squares(const T* __restrict__ p, int n) {
   for (; i + 3 * kStep < whole; i += 4 * kStep) {
     u32x4 v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = load16(p + i + u * kStep);
+    for (int u = 0; u < 4; ++u) v[u] = load_<PAST>(p + i + u * kStep);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -71,7 +87,7 @@ __device__ __forceinline__ double squares(const T* __restrict__ p, int n) {
       }
   }
   for (; i < whole; i += kStep) {
-    const u32x4 v = load16(p + i);
+    const u32x4 v = load_<PAST>(p + i);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const double x = Elem<T>::get(v, j);
@@ -96,6 +112,7 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
   return s;
 }
 
+template <bool PAST>
 __global__ __launch_bounds__(kThreads) void norm_partials_kernel(
     const TensorList l, double* __restrict__ partials) {
   __shared__ double lds[kThreads / 64];
@@ -107,21 +124,21 @@ __global__ __launch_bounds__(kThreads) void norm_partials_kernel(
     const int n = (int)min((long)kChunk, l.numel[t] - start);
     switch (l.type[t]) {
       case 0:
-        acc += squares(static_cast<const float*>(l.src[t]) + start, n);
+        acc += squares<PAST>(static_cast<const float*>(l.src[t]) + start, n);
         break;
       case 1:
-        acc += squares(
+        acc += squares<PAST>(
             static_cast<const __hip_bfloat16*>(l.src[t]) + start, n);
         break;
       default:
-        acc += squares(static_cast<const __half*>(l.src[t]) + start, n);
+        acc += squares<PAST>(static_cast<const __half*>(l.src[t]) + start, n);
     }
   }
   const double s = block_sum(acc, lds);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-template <typename T>
+template <bool PAST, typename T>
 __device__ __forceinline__ void scaled(const T* p, T* q, int n, float f) {
   constexpr int V = Elem<T>::kVec;
   constexpr int kStep = kThreads * V;
@@ -130,21 +147,21 @@ __device__ __forceinline__ void scaled(const T* p, T* q, int n, float f) {
   for (; i + 3 * kStep < whole; i += 4 * kStep) {
     u32x4 v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = load16(p + i + u * kStep);
+    for (int u = 0; u < 4; ++u) v[u] = load_<PAST>(p + i + u * kStep);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float x[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) x[j] = Elem<T>::get(v[u], j) * f;
-      store16(q + i + u * kStep, Elem<T>::pack(x));
+      store_<PAST>(q + i + u * kStep, Elem<T>::pack(x));
     }
   }
   for (; i < whole; i += kStep) {
-    const u32x4 v = load16(p + i);
+    const u32x4 v = load_<PAST>(p + i);
     float x[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) x[j] = Elem<T>::get(v, j) * f;
-    store16(q + i, Elem<T>::pack(x));
+    store_<PAST>(q + i, Elem<T>::pack(x));
   }
   if (whole + (int)threadIdx.x < n)
     q[whole + threadIdx.x] =
@@ -152,6 +169,7 @@ __device__ __forceinline__ void scaled(const T* p, T* q, int n, float f) {
 }
 
 // Also the whole of the norm alone, with no tensors in the list.
+template <bool PAST>
 __global__ __launch_bounds__(kThreads) void clip_scale_list_kernel(
     const TensorList l, const double* __restrict__ partials, int npartials,
     double max_norm, double eps, float* __restrict__ norm_out) {
@@ -173,15 +191,15 @@ __global__ __launch_bounds__(kThreads) void clip_scale_list_kernel(
     const int n = (int)min((long)kChunk, l.numel[t] - start);
     switch (l.type[t]) {
       case 0:
-        scaled(static_cast<const float*>(l.src[t]) + start,
+        scaled<PAST>(static_cast<const float*>(l.src[t]) + start,
                static_cast<float*>(l.dst[t]) + start, n, f);
         break;
       case 1:
-        scaled(static_cast<const __hip_bfloat16*>(l.src[t]) + start,
+        scaled<PAST>(static_cast<const __hip_bfloat16*>(l.src[t]) + start,
                static_cast<__hip_bfloat16*>(l.dst[t]) + start, n, f);
         break;
       default:
-        scaled(static_cast<const __half*>(l.src[t]) + start,
+        scaled<PAST>(static_cast<const __half*>(l.src[t]) + start,
                static_cast<__half*>(l.dst[t]) + start, n, f);
     }
   }
@@ -240,8 +258,10 @@ torch::Tensor clip_list(const std::vector<torch::Tensor>& src,
   const auto stream = current_stream();
 
   std::vector<TensorList> lists;
+  long bytes = 0;
   for (size_t i = 0; i < src.size(); ++i) {
     if (src[i].numel() == 0) continue;
+    bytes += src[i].numel() * src[i].element_size();
     const long chunks = (src[i].numel() + kChunk - 1) / kChunk;
     if (lists.empty() || lists.back().count == kMaxTensors) {
       lists.emplace_back();
@@ -266,9 +286,12 @@ torch::Tensor clip_list(const std::vector<torch::Tensor>& src,
   auto partials =
       torch::empty({std::max(at.back(), 1)}, opts.dtype(torch::kDouble));
   double* pp = partials.data_ptr<double>();
+  const bool past = bytes >= kPastBytes;
   for (size_t i = 0; i < lists.size(); ++i) {
-    hipLaunchKernelGGL(norm_partials_kernel, dim3(at[i + 1] - at[i]),
-                       dim3(kThreads), 0, stream, lists[i], pp + at[i]);
+    const auto kernel =
+        past ? norm_partials_kernel<true> : norm_partials_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(at[i + 1] - at[i]), dim3(kThreads), 0,
+                       stream, lists[i], pp + at[i]);
     CHECK_HIP(hipGetLastError());
   }
   if (dst.empty() || lists.empty()) {
@@ -278,8 +301,10 @@ torch::Tensor clip_list(const std::vector<torch::Tensor>& src,
   }
   for (size_t i = lists.size(); i-- > 0;) {
     const int chunks = lists[i].first[lists[i].count];
-    hipLaunchKernelGGL(clip_scale_list_kernel,
-                       dim3(std::max(1, std::min(chunks, kMaxBlocks))),
+    const auto kernel =
+        past ? clip_scale_list_kernel<true> : clip_scale_list_kernel<false>;
+    hipLaunchKernelGGL(kernel,
+                       dim3(std::max(1, std::min(chunks, kMaxScaleBlocks))),
                        dim3(kThreads), 0, stream, lists[i], pp, at.back(),
                        max_norm, eps,
                        i == 0 ? norm.data_ptr<float>() : nullptr);
@@ -301,9 +326,26 @@ std::tuple<std::vector<torch::Tensor>, torch::Tensor> clip_grads(
   TORCH_CHECK(!grads.empty(), "no gradients");
   c10::DeviceGuard guard(grads[0].device());
   const auto src = as_dense(grads);
+  // One buffer for all of them, each at a multiple of 256 bytes: an
+  // allocation for each costs as much host time as all the rest.
+  std::vector<long> at(1, 0);
+  for (const auto& t : src)
+    at.push_back((at.back() + t.numel() * (long)t.element_size() + 255) &
+                 ~255L);
+  const auto buffer = torch::empty(
+      {at.back()}, torch::TensorOptions().device(src[0].device()).dtype(
+                       torch::kByte));
   std::vector<torch::Tensor> dst;
   dst.reserve(src.size());
-  for (const auto& t : src) dst.push_back(torch::empty_like(t));
+  for (size_t i = 0; i < src.size(); ++i) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(buffer.storage()), buffer.key_set(), src[i].dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(
+        at[i] / (long)src[i].element_size());
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(src[i].sizes(),
+                                                   src[i].strides());
+    dst.push_back(std::move(t));
+  }
   auto norm = clip_list(src, dst, max_norm, eps);
   return {std::move(dst), std::move(norm)};
 }

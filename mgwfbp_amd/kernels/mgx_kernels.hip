@@ -37,6 +37,8 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kBlock = 256;          // 4 wave64s
 constexpr long kChunk = 1 << 16;     // elements per chunk (64K)
 constexpr int kMaxGrid = 2048;       // 256 CUs * 8 blocks
@@ -73,7 +75,29 @@ struct Chunk {
 // order and folds min(1, max_norm / (norm + eps)) into grad_scale, so
 // clipping costs one read of the gradients and writes none of them. Block
 // 0 leaves the norm of the scaled gradients in norm_out.
-template <bool CLIP>
+//
+// PAST (with CLIP): every access goes past the 256 MB cache, for more than
+// it holds.
+template <bool PAST>
+__device__ __forceinline__ float4 sgd_load(const float* p) {
+  if constexpr (PAST) {
+    const f32x4 v =
+        __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+    return make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    return *reinterpret_cast<const float4*>(p);
+  }
+}
+template <bool PAST>
+__device__ __forceinline__ void sgd_store(float* p, const float4& v) {
+  if constexpr (PAST)
+    __builtin_nontemporal_store(f32x4{v.x, v.y, v.z, v.w},
+                                reinterpret_cast<f32x4*>(p));
+  else
+    *reinterpret_cast<float4*>(p) = v;
+}
+
+template <bool CLIP, bool PAST>
 __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
     const Chunk* __restrict__ chunks, int nchunks,
     const TensorTriple* __restrict__ tensors, float lr,
@@ -96,13 +120,18 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
     const double f = max_norm / (norm + eps);
     if (!(f >= 1.)) grad_scale = (float)(grad_scale * f);  // NaN stays one
   }
-  for (int k = blockIdx.x; k < nchunks; k += gridDim.x) {
-    // CLIP goes from the last chunk back: what the norm's pass read last
-    // is still in the 256 MB cache
-    const int c = CLIP ? nchunks - 1 - k : k;
-    const Chunk ck = chunks[c];
+  // CLIP takes a chunk in four pieces, so that a block for each fills the
+  // card, and goes from the last one back: what the norm's pass read last is
+  // still in the 256 MB cache.
+  constexpr int kPieces = CLIP ? 4 : 1;
+  const int npieces = nchunks * kPieces;
+  for (int k = blockIdx.x; k < npieces; k += gridDim.x) {
+    const int c = CLIP ? npieces - 1 - k : k;
+    Chunk ck = chunks[c / kPieces];
+    ck.start += c % kPieces * (kChunk / kPieces);
     const TensorTriple t = tensors[ck.tensor_idx];
-    const long n = min(kChunk, t.numel - ck.start);
+    const long n = min(kChunk / kPieces, t.numel - ck.start);
+    if (CLIP && n <= 0) continue;
     float* __restrict__ p = t.p + ck.start;
     float* __restrict__ g = t.g + ck.start;
     float* __restrict__ m = t.m ? t.m + ck.start : nullptr;
@@ -113,14 +142,14 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
     const long step = (long)blockDim.x * 4L;
     long i = threadIdx.x * 4L;
     for (; i + step < nvec; i += 2 * step) {
-      float4 pv0 = *reinterpret_cast<float4*>(p + i);
-      float4 gv0 = *reinterpret_cast<float4*>(g + i);
-      float4 pv1 = *reinterpret_cast<float4*>(p + i + step);
-      float4 gv1 = *reinterpret_cast<float4*>(g + i + step);
+      float4 pv0 = sgd_load<PAST>(p + i);
+      float4 gv0 = sgd_load<PAST>(g + i);
+      float4 pv1 = sgd_load<PAST>(p + i + step);
+      float4 gv1 = sgd_load<PAST>(g + i + step);
       float4 mv0, mv1;
       if (m) {
-        mv0 = *reinterpret_cast<float4*>(m + i);
-        mv1 = *reinterpret_cast<float4*>(m + i + step);
+        mv0 = sgd_load<PAST>(m + i);
+        mv1 = sgd_load<PAST>(m + i + step);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -147,26 +176,26 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
         pv.z -= lr * dp2; pv.w -= lr * dp3;
       }
       if (m) {
-        *reinterpret_cast<float4*>(m + i) = mv0;
-        *reinterpret_cast<float4*>(m + i + step) = mv1;
+        sgd_store<PAST>(m + i, mv0);
+        sgd_store<PAST>(m + i + step, mv1);
       }
-      *reinterpret_cast<float4*>(p + i) = pv0;
-      *reinterpret_cast<float4*>(p + i + step) = pv1;
+      sgd_store<PAST>(p + i, pv0);
+      sgd_store<PAST>(p + i + step, pv1);
     }
     for (; i < nvec; i += step) {
-      float4 pv = *reinterpret_cast<float4*>(p + i);
-      float4 gv = *reinterpret_cast<float4*>(g + i);
+      float4 pv = sgd_load<PAST>(p + i);
+      float4 gv = sgd_load<PAST>(g + i);
       float dp0 = gv.x * grad_scale + wd * pv.x;
       float dp1 = gv.y * grad_scale + wd * pv.y;
       float dp2 = gv.z * grad_scale + wd * pv.z;
       float dp3 = gv.w * grad_scale + wd * pv.w;
       if (m) {
-        float4 mv = *reinterpret_cast<float4*>(m + i);
+        float4 mv = sgd_load<PAST>(m + i);
         mv.x = momentum * mv.x + (1.f - dampening) * dp0;
         mv.y = momentum * mv.y + (1.f - dampening) * dp1;
         mv.z = momentum * mv.z + (1.f - dampening) * dp2;
         mv.w = momentum * mv.w + (1.f - dampening) * dp3;
-        *reinterpret_cast<float4*>(m + i) = mv;
+        sgd_store<PAST>(m + i, mv);
         if (nesterov) {
           dp0 += momentum * mv.x; dp1 += momentum * mv.y;
           dp2 += momentum * mv.z; dp3 += momentum * mv.w;
@@ -176,7 +205,7 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
       }
       pv.x -= lr * dp0; pv.y -= lr * dp1;
       pv.z -= lr * dp2; pv.w -= lr * dp3;
-      *reinterpret_cast<float4*>(p + i) = pv;
+      sgd_store<PAST>(p + i, pv);
     }
     for (long i = nvec + threadIdx.x; i < n; i += blockDim.x) {
       float dp = g[i] * grad_scale + wd * p[i];
@@ -193,6 +222,7 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
 // Sums of squares of the gradients, one for each block, in 64 bits: they
 // neither overflow nor lose the squares of small gradients, and cost
 // nothing beside the loads.
+template <bool PAST>
 __global__ __launch_bounds__(kBlock) void sgd_norm_partials_kernel(
     const Chunk* __restrict__ chunks, int nchunks,
     const TensorTriple* __restrict__ tensors,
@@ -210,7 +240,7 @@ __global__ __launch_bounds__(kBlock) void sgd_norm_partials_kernel(
       float4 v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        v[u] = *reinterpret_cast<const float4*>(g + i + u * step);
+        v[u] = sgd_load<PAST>(g + i + u * step);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         a0 = fma((double)v[u].x, (double)v[u].x, a0);
@@ -220,7 +250,7 @@ __global__ __launch_bounds__(kBlock) void sgd_norm_partials_kernel(
       }
     }
     for (; i < nvec; i += step) {
-      const float4 v = *reinterpret_cast<const float4*>(g + i);
+      const float4 v = sgd_load<PAST>(g + i);
       a0 = fma((double)v.x, (double)v.x, a0);
       a1 = fma((double)v.y, (double)v.y, a1);
       a0 = fma((double)v.z, (double)v.z, a0);
@@ -507,7 +537,7 @@ void multi_tensor_sgd(torch::Tensor t_tensors, torch::Tensor t_chunks,
   const float* lr_ptr =
       lr_buf.defined() && lr_buf.numel() > 0
           ? lr_buf.data_ptr<float>() : nullptr;
-  hipLaunchKernelGGL(multi_tensor_sgd_kernel<false>, dim3(grid_for(nchunks)),
+  hipLaunchKernelGGL((multi_tensor_sgd_kernel<false, false>), dim3(grid_for(nchunks)),
                      dim3(kBlock), 0, c10::hip::getCurrentHIPStream().stream(),
                      reinterpret_cast<const Chunk*>(t_chunks.data_ptr()),
                      (int)nchunks,
@@ -537,16 +567,21 @@ torch::Tensor multi_tensor_sgd_clipped(
   const int nparts = std::max(1, std::min((int)nchunks, 1024));
   auto partials = torch::empty({nparts}, opts.dtype(torch::kDouble));
   auto norm = torch::empty({}, opts.dtype(torch::kFloat));
-  hipLaunchKernelGGL(sgd_norm_partials_kernel, dim3(nparts), dim3(kBlock), 0,
-                     stream, chunks, (int)nchunks, tensors,
-                     partials.data_ptr<double>());
+  // what the chunks can hold at most; the update past the cache from 128 MB
+  // of parameters on
+  const bool past = nchunks * kChunk * (long)sizeof(float) >= (128L << 20);
+  const auto sums = past ? sgd_norm_partials_kernel<true>
+                         : sgd_norm_partials_kernel<false>;
+  const auto update = past ? multi_tensor_sgd_kernel<true, true>
+                           : multi_tensor_sgd_kernel<true, false>;
+  hipLaunchKernelGGL(sums, dim3(nparts), dim3(kBlock), 0, stream, chunks,
+                     (int)nchunks, tensors, partials.data_ptr<double>());
   CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(multi_tensor_sgd_kernel<true>,
-                     dim3(std::max(1, grid_for(nchunks))), dim3(kBlock), 0,
-                     stream, chunks, (int)nchunks, tensors, (float)lr, lr_ptr,
-                     (float)momentum, (float)dampening, nesterov,
-                     (float)grad_scale, partials.data_ptr<double>(), nparts,
-                     max_norm, eps, norm.data_ptr<float>());
+  hipLaunchKernelGGL(update, dim3(std::max(1, grid_for(4 * nchunks))),
+                     dim3(kBlock), 0, stream, chunks, (int)nchunks, tensors,
+                     (float)lr, lr_ptr, (float)momentum, (float)dampening,
+                     nesterov, (float)grad_scale, partials.data_ptr<double>(),
+                     nparts, max_norm, eps, norm.data_ptr<float>());
   CHECK_HIP(hipGetLastError());
   return norm;
 }
