@@ -44,10 +44,10 @@ __device__ __forceinline__ long token_at(const void* p, bool wide, long i) {
 }
 
 // The first `cols` elements of a vector; the rest is zero.
-template <typename T>
+template <typename T, bool PAST = false>
 __device__ __forceinline__ u32x4 load_cols(const T* p, int cols) {
   constexpr int V = Elem<T>::kVec;
-  if (cols >= V) return load16(p);
+  if (cols >= V) return PAST ? load16_past(p) : load16(p);
   float f[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) f[j] = j < cols ? Elem<T>::up(p[j]) : 0.f;
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(kThreads) void sum_runs_kernel(
     for (int u = 0; u < U; ++u)
       if (j0 + u < n && cols > 0) {
         const uint32_t p = __builtin_amdgcn_readlane(pos, min(j0 + u, 63));
-        f[u] = load_cols(dout + (long)p * row_stride + col, cols);
+        f[u] = load_cols<T, true>(dout + (long)p * row_stride + col, cols);
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -603,10 +603,27 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   const long row = (long)r.slices * 64 * V;
   const float* p = pieces + ((long)slice * 64 + lane) * V;
-  // piece 0 is the run's beginning, piece i the first of chunk + i
-  for (int i = wave; i <= more; i += kWaves) {
-    const float* q =
-        p + (i == 0 ? (long)chunk * 2 + 1 : ((long)chunk + i) * 2) * row;
+  // piece 0 is the run's beginning, piece i the first of chunk + i; four of
+  // them under way at once
+  const auto piece = [&](int i) {
+    return p + (i == 0 ? (long)chunk * 2 + 1 : ((long)chunk + i) * 2) * row;
+  };
+  int i = wave;
+  for (; i + 3 * kWaves <= more; i += 4 * kWaves) {
+    float f[4][V];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* q = piece(i + u * kWaves);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[u][j] = q[j];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += f[u][j];
+  }
+  for (; i <= more; i += kWaves) {
+    const float* q = piece(i);
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] += q[j];
   }

@@ -27,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxTensors = 120;       // their addresses fit 4 KB of arguments
 constexpr int kChunk = 16384;          // elements of one block's turn
 constexpr int kMaxBlocks = 1024;       // that leave a partial sum
-constexpr int kMaxScaleBlocks = 2048;  // 8 blocks of 4 waves on each CU
+constexpr int kMaxScaleBlocks = 2048;  // that stay and take several chunks
 
 struct TensorList {
   const void* src[kMaxTensors];
@@ -183,8 +183,10 @@ __global__ __launch_bounds__(kThreads) void clip_scale_list_kernel(
   const float f = c >= 1. ? 1.f : (float)c;   // a NaN stays one
   const int chunks = l.first[l.count];
   // From the last chunk back: what the first launch read last is still in
-  // the 256 MB cache.
-  for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+  // the 256 MB cache. Past the cache in order, and a block for each chunk:
+  // 300M elements take 311 us by 2048 blocks from the back, 295 us so.
+  for (int k = blockIdx.x; k < chunks; k += gridDim.x) {
+    const int c = PAST ? k : chunks - 1 - k;
     const int t = tensor_of(l, c);
     if (f == 1.f && l.src[t] == l.dst[t]) continue;
     const long start = (long)(c - l.first[t]) * kChunk;
@@ -304,7 +306,8 @@ torch::Tensor clip_list(const std::vector<torch::Tensor>& src,
     const auto kernel =
         past ? clip_scale_list_kernel<true> : clip_scale_list_kernel<false>;
     hipLaunchKernelGGL(kernel,
-                       dim3(std::max(1, std::min(chunks, kMaxScaleBlocks))),
+                       dim3(std::max(1, past ? chunks
+                                         : std::min(chunks, kMaxScaleBlocks))),
                        dim3(kThreads), 0, stream, lists[i], pp, at.back(),
                        max_norm, eps,
                        i == 0 ? norm.data_ptr<float>() : nullptr);

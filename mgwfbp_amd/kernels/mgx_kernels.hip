@@ -121,12 +121,12 @@ __global__ __launch_bounds__(kBlock) void multi_tensor_sgd_kernel(
     if (!(f >= 1.)) grad_scale = (float)(grad_scale * f);  // NaN stays one
   }
   // CLIP takes a chunk in four pieces, so that a block for each fills the
-  // card, and goes from the last one back: what the norm's pass read last is
-  // still in the 256 MB cache.
+  // card, and goes from the last one back unless it goes past the 256 MB
+  // cache: what the norm's pass read last is still there.
   constexpr int kPieces = CLIP ? 4 : 1;
   const int npieces = nchunks * kPieces;
   for (int k = blockIdx.x; k < npieces; k += gridDim.x) {
-    const int c = CLIP ? npieces - 1 - k : k;
+    const int c = CLIP && !PAST ? npieces - 1 - k : k;
     Chunk ck = chunks[c / kPieces];
     ck.start += c % kPieces * (kChunk / kPieces);
     const TensorTriple t = tensors[ck.tensor_idx];
@@ -577,7 +577,8 @@ torch::Tensor multi_tensor_sgd_clipped(
   hipLaunchKernelGGL(sums, dim3(nparts), dim3(kBlock), 0, stream, chunks,
                      (int)nchunks, tensors, partials.data_ptr<double>());
   CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(update, dim3(std::max(1, grid_for(4 * nchunks))),
+  hipLaunchKernelGGL(update, dim3(std::max(1, past ? 4 * (int)nchunks
+                                         : grid_for(4 * nchunks))),
                      dim3(kBlock), 0, stream, chunks, (int)nchunks, tensors,
                      (float)lr, lr_ptr, (float)momentum, (float)dampening,
                      nesterov, (float)grad_scale, partials.data_ptr<double>(),
