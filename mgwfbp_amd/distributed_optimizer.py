@@ -476,10 +476,12 @@ class _DistributedOptimizer(torch.optim.Optimizer):
             # per-group LRs diverged (user schedule): the single-launch
             # fused kernel carries one LR — use the torch loop instead
         if max_grad_norm is not None:
-            from .kernels import grad_clip
-            grad_clip.clip_grad_norm_(
-                [p for g in self.param_groups for p in g['params']],
-                max_grad_norm)
+            params = [p for g in self.param_groups for p in g['params']]
+            if settings.USE_HIP_KERNELS:
+                from .kernels import grad_clip
+                grad_clip.clip_grad_norm_(params, max_grad_norm)
+            else:
+                torch.nn.utils.clip_grad_norm_(params, max_grad_norm)
         return super(self.__class__, self).step(closure)
 
     def zero_grad(self, set_to_none=False):

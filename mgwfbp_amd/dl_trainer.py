@@ -33,7 +33,8 @@ from torch.utils.data.distributed import DistributedSampler
 from . import models
 from . import settings
 from . import data as mgx_data
-from .kernels.token_loss import MgxCrossEntropyLoss, token_log_probs
+from .kernels.token_loss import (MgxCrossEntropyLoss, token_log_probs,
+                                 token_log_probs_reference)
 from .settings import logger
 
 # MIOpen autotune. Measured on MI355X (resnet50 bs128 bf16 NHWC):
@@ -575,8 +576,9 @@ class DLTrainer:
                     if x.size(0) != self.net.batch_size:
                         continue
                     out, _ = self.net(x, hidden)
-                    r = token_log_probs(out, y,
-                                        top_k=min(5, self.net.ntokens))
+                    score = (token_log_probs if settings.USE_HIP_KERNELS
+                             else token_log_probs_reference)
+                    r = score(out, y, top_k=min(5, self.net.ntokens))
                     # accumulated on the device, read back at the end
                     total_loss -= r.log_probs.mean()
                     total_entropy += r.entropy.mean()

@@ -667,9 +667,9 @@ torch::Tensor gather_rows(const torch::Tensor& weight,
     // four vectors a thread once they still fill the card
     const bool four = n * vecs >= 4L * kThreads * 1024;
     const long blocks = ceil_div(n * vecs, kThreads * (four ? 4 : 1));
-    TORCH_CHECK_VALUE(blocks < (1L << 31), "too many tokens");
+    const dim3 grid = grid_of(blocks, kThreads, "tokens");
     const auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, stream,
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream,
                          tokens.data_ptr(), is_wide(tokens), n,
                          static_cast<const T*>(weight.data_ptr()),
                          (long)weight.stride(0), (long)weight.size(0),
@@ -756,9 +756,9 @@ torch::Tensor weight_grad(const torch::Tensor& tokens,
       using T = decltype(z);
       const long slices = ceil_div(dim, 64L * Elem<T>::kVec);
       const long blocks = ceil_div(vocab, kOwned) * slices;
-      TORCH_CHECK_VALUE(blocks < (1L << 31), "the table is too large");
-      hipLaunchKernelGGL(owned_rows_kernel<T>, dim3(blocks), dim3(kThreads),
-                         0, current_stream(), tokens.data_ptr(),
+      hipLaunchKernelGGL(owned_rows_kernel<T>,
+                         grid_of(blocks, kThreads, "rows of the table"),
+                         dim3(kThreads), 0, current_stream(), tokens.data_ptr(),
                          is_wide(tokens), (int)n, vocab, padding, (int)dim,
                          (int)slices, scale,
                          static_cast<const T*>(dout.data_ptr()),
@@ -805,7 +805,7 @@ torch::Tensor weight_grad(const torch::Tensor& tokens,
     r.dim = (int)dim;
     r.scale = scale;
     const long waves = (long)r.chunks * r.slices;
-    TORCH_CHECK_VALUE(waves < (1L << 31), "too many tokens");
+    const dim3 joins = grid_of(waves, kThreads, "tokens");
     auto pieces = torch::empty(
         {r.chunks > 1 ? waves * 2 * 64 * Elem<T>::kVec : 1},
         dout.options().dtype(torch::kFloat));
@@ -818,7 +818,7 @@ torch::Tensor weight_grad(const torch::Tensor& tokens,
                        (long)dout.stride(0), pg, pp);
     CHECK_HIP(hipGetLastError());
     if (r.chunks > 1) {
-      hipLaunchKernelGGL(join_runs_kernel<T>, dim3(waves), dim3(kThreads), 0,
+      hipLaunchKernelGGL(join_runs_kernel<T>, joins, dim3(kThreads), 0,
                          stream, r, pp, pg);
       CHECK_HIP(hipGetLastError());
     }

@@ -271,8 +271,7 @@ torch::Tensor clip_list(const std::vector<torch::Tensor>& src,
       lists.back().first[0] = 0;
     }
     TensorList& l = lists.back();
-    TORCH_CHECK(l.first[l.count] + chunks < (1L << 31),
-                "gradients too large for one call");
+    grid_of(l.first[l.count] + chunks, kThreads, "gradients");
     l.src[l.count] = src[i].data_ptr();
     l.dst[l.count] = dst.empty() ? nullptr : dst[i].data_ptr();
     l.numel[l.count] = src[i].numel();

@@ -138,6 +138,13 @@ void with_elem(at::ScalarType t, const char* what, F&& f) {
   }
 }
 
+// A launch counts its threads in 32 bits.
+inline dim3 grid_of(long blocks, long threads, const char* what) {
+  TORCH_CHECK_VALUE(blocks * threads < (1L << 32), "too many ", what,
+                    " for one call");
+  return dim3((unsigned)blocks);
+}
+
 inline hipStream_t current_stream() {
   return c10::hip::getCurrentHIPStream().stream();
 }

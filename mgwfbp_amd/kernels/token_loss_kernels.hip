@@ -1053,7 +1053,6 @@ void launch_stats(const torch::Tensor& x, const torch::Tensor& targets,
     w.slice = (int)(ceil_div(ceil_div(vocab, splits), step) * step);
   splits = ceil_div(vocab, w.slice);
   w.splits = (int)splits;
-  TORCH_CHECK_VALUE(rows * splits < (1L << 31), "too many rows");
   const auto stream = current_stream();
   const auto opts = torch::TensorOptions().device(x.device());
   torch::Tensor stats, keys;
@@ -1069,16 +1068,17 @@ void launch_stats(const torch::Tensor& x, const torch::Tensor& targets,
   const bool held = vocab >= kHeldLeast &&
       with_slice(w.slice / Elem<T>::kVec, [&](auto block, auto nv) {
         hipLaunchKernelGGL((held_stats_kernel<T, block.value, nv.value, TOP>),
-                           dim3(rows * splits), dim3(block.value), 0, stream,
-                           px, w, out, ps, pk);
+                           grid_of(rows * splits, block.value, "rows"),
+                           dim3(block.value), 0, stream, px, w, out, ps, pk);
       });
   if (!held)
-    hipLaunchKernelGGL((row_stats_kernel<T, TOP>), dim3(rows * splits),
+    hipLaunchKernelGGL((row_stats_kernel<T, TOP>),
+                       grid_of(rows * splits, kThreads, "rows"),
                        dim3(kThreads), 0, stream, px, w, out, ps, pk);
   CHECK_HIP(hipGetLastError());
   if (splits > 1) {
-    hipLaunchKernelGGL((join_rows_kernel<T, TOP>), dim3(rows),
-                       dim3(kThreads), 0, stream, px, w, out, ps, pk);
+    hipLaunchKernelGGL((join_rows_kernel<T, TOP>),
+                       grid_of(rows, kThreads, "rows"), dim3(kThreads), 0, stream, px, w, out, ps, pk);
     CHECK_HIP(hipGetLastError());
   }
 }
@@ -1102,7 +1102,7 @@ torch::Tensor loss_and_grad(const torch::Tensor& x,
                             bool mean, float* share, const RowOut& out) {
   torch::Tensor grad;
   const long rows = x.size(0);
-  if (rows == 0 || rows >= (1L << 31) || x.size(1) < kHeldLeast) return grad;
+  if (rows == 0 || x.size(1) < kHeldLeast) return grad;
   const auto stream = current_stream();
   with_elem(x.scalar_type(), "logits", [&](auto z) {
     using T = decltype(z);
@@ -1116,7 +1116,8 @@ torch::Tensor loss_and_grad(const torch::Tensor& x,
       }
       grad = torch::empty({rows, x.size(1)}, x.options());
       hipLaunchKernelGGL((row_loss_kernel<T, block.value, nv.value>),
-                         dim3(rows), dim3(block.value), 0, stream,
+                         grid_of(rows, block.value, "rows"),
+                         dim3(block.value), 0, stream,
                          static_cast<const T*>(x.data_ptr()), w, out, rows,
                          mean, count ? share : nullptr,
                          static_cast<T*>(grad.data_ptr()));
@@ -1148,14 +1149,12 @@ torch::Tensor grad_of(const torch::Tensor& x, const GradIn& in,
                          0, stream, px, (long)x.stride(0), vocab, (int)parts,
                          slice, rows * parts, in, py);
     } else {
-      TORCH_CHECK_VALUE(rows * parts < (1L << 31), "too many rows");
+      const dim3 grid = grid_of(rows * parts, kThreads, "rows");
       if (in.grad_entropy != nullptr)
-        hipLaunchKernelGGL((row_grad_kernel<T, true>), dim3(rows * parts),
-                           dim3(kThreads), 0, stream, px, (long)x.stride(0),
+        hipLaunchKernelGGL((row_grad_kernel<T, true>), grid, dim3(kThreads), 0, stream, px, (long)x.stride(0),
                            vocab, (int)parts, slice, in, py);
       else
-        hipLaunchKernelGGL((row_grad_kernel<T, false>), dim3(rows * parts),
-                           dim3(kThreads), 0, stream, px, (long)x.stride(0),
+        hipLaunchKernelGGL((row_grad_kernel<T, false>), grid, dim3(kThreads), 0, stream, px, (long)x.stride(0),
                            vocab, (int)parts, slice, in, py);
     }
     CHECK_HIP(hipGetLastError());

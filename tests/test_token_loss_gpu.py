@@ -344,6 +344,54 @@ def test_strides_shapes_and_neighbours(kind):
                        kind)
 
 
+@pytest.mark.parametrize('kind', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,vocab,k', [
+    (2, 300001, 64), (1, 1100003, 0), (3, 600007, 64), (600, 131073, 3),
+    (2, 2100001, 20)])
+def test_long_rows(rows, vocab, k, kind):
+    """Rows that no block holds: split, and streamed where the slices are
+    still too long."""
+    x, t = _make(rows, vocab, kind, seed=17)
+    x[0, ::7] = NEG
+    t[0] = 1
+    x.requires_grad_(True)
+    r = tl.token_log_probs(x, t, top_k=k)
+    far = 4 * REL                        # a thread's share is V / 4096 here
+    for i in range(0, rows, 97):
+        log, p, h = _exact(x[i:i + 1])
+        assert abs(float(r.log_probs[i].detach())
+                   - float(log[0, t[i]])) <= far
+        assert abs(float(r.entropy[i].detach()) - float(h[0])) <= far
+        ids = torch.sort(x[i].detach(), descending=True,
+                         stable=True)[1][:k]
+        assert torch.equal(r.top_ids[i], ids)
+    loss = tl.cross_entropy(x, t)
+    assert abs(float(loss.detach())
+               + float(r.log_probs.detach().mean())) <= far
+    got, = torch.autograd.grad(loss, x)
+    for i in range(0, rows, 97):
+        log, p, _ = _exact(x[i:i + 1])
+        p[0, t[i]] -= 1.0
+        want = p / rows
+        off = (got[i].double() - want[0]).abs()
+        most = torch.finfo(kind).eps / 2 * want[0].abs() + \
+            2 * far * want[0].abs() + 4 * U / rows
+        assert bool((off <= most).all())
+
+
+def test_more_rows_than_a_launch_takes():
+    """Refused, not cut short: 2^24 blocks of 256 threads are one thread too
+    many."""
+    x = torch.zeros(1, 2, dtype=torch.bfloat16, device='cuda')
+    x = x.expand(1 << 24, 2)
+    t = torch.zeros(1 << 24, dtype=torch.int32, device='cuda')
+    with pytest.raises(ValueError):
+        tl.token_log_probs(x, t)
+    r = tl.token_log_probs(x[:-1], t[:-1])
+    assert abs(float(r.entropy[-1]) - 0.6931472) < 1e-6
+    assert bool((r.log_probs == r.log_probs[0]).all())
+
+
 def test_one_row_and_none():
     x, _ = _make(1, 50, torch.float32)
     v = x[0]
