@@ -246,9 +246,10 @@ __global__ __launch_bounds__(1024) void sort_and_clear_kernel(
   }
 }
 
-// More tokens: for each digit, counts by tile, their exclusive sums (digit
-// by digit, tile by tile), and a stable scatter.
-constexpr int kTileItems = 16;
+// More tokens: for each digit of 8 bits or less, counts by tile, their
+// exclusive sums for each digit over the tiles, and a stable scatter. A
+// pass over 131072 tokens takes 20 us with dW's clearing and 18 without.
+constexpr int kTileItems = 8;
 constexpr int kTile = kThreads * kTileItems;
 
 struct SortIn {            // the tokens, or what the last pass wrote
@@ -287,38 +288,34 @@ __global__ __launch_bounds__(kThreads) void tile_counts_kernel(
   counts[(long)threadIdx.x * tiles + blockIdx.x] = mine[threadIdx.x];
 }
 
-__global__ __launch_bounds__(1024) void scan_counts_kernel(
-    int* __restrict__ counts, int n) {
-  __shared__ int sums[16];
-  const int each = (n + 1023) / 1024;
-  const int from = min(n, (int)threadIdx.x * each);
-  const int to = min(n, from + each);
-  int s = 0;
-  for (int i = from; i < to; ++i) s += counts[i];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int run = s;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(run, off, 64);
-    if (lane >= off) run += o;
+// Block d: the exclusive sums of digit d's counts over the tiles, and their
+// total.
+__global__ __launch_bounds__(kThreads) void scan_counts_kernel(
+    int* __restrict__ counts, int tiles, int* __restrict__ totals) {
+  __shared__ int sums[4];
+  __shared__ int last;
+  int* __restrict__ mine = counts + (long)blockIdx.x * tiles;
+  int before = 0;
+  for (int from = 0; from < tiles; from += kThreads) {
+    const int i = from + threadIdx.x;
+    const int c = i < tiles ? mine[i] : 0;
+    const int at = before + exclusive_256(c, sums);
+    if (i < tiles) mine[i] = at;
+    if (threadIdx.x == kThreads - 1) last = at + c;
+    __syncthreads();
+    before = last;
+    __syncthreads();                   // sums and last are free again
   }
-  if (lane == 63) sums[wave] = run;
-  __syncthreads();
-  run -= s;
-  for (int w = 0; w < wave; ++w) run += sums[w];
-  for (int i = from; i < to; ++i) {
-    const int c = counts[i];
-    counts[i] = run;
-    run += c;
-  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
 __global__ __launch_bounds__(kThreads) void tile_scatter_kernel(
     SortIn in, long n, int tiles, int shift, int bits,
-    const int* __restrict__ counts, uint32_t* __restrict__ keys,
-    uint32_t* __restrict__ positions) {
+    const int* __restrict__ counts, const int* __restrict__ totals,
+    uint32_t* __restrict__ keys, uint32_t* __restrict__ positions) {
   constexpr int kWaves = kThreads / 64;
   __shared__ int mine[kWaves * kDigits];
+  __shared__ int sums[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int i = threadIdx.x; i < kWaves * kDigits; i += kThreads) mine[i] = 0;
   __syncthreads();
@@ -333,8 +330,11 @@ __global__ __launch_bounds__(kThreads) void tile_scatter_kernel(
   int rank[kTileItems];
   wave_ranks<uint32_t, kTileItems>(item, shift, bits, mine + wave * kDigits,
                                    rank);
-  __syncthreads();
-  int at = counts[(long)threadIdx.x * tiles + blockIdx.x];
+  // what stands before this tile's share of digit threadIdx.x: the lower
+  // digits, and the same digit in the tiles before (the sum's barrier also
+  // orders the ranks)
+  int at = exclusive_256(totals[threadIdx.x], sums) +
+      counts[(long)threadIdx.x * tiles + blockIdx.x];
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     const int c = mine[w * kDigits + threadIdx.x];
@@ -711,7 +711,8 @@ void launch_big_sort(const torch::Tensor& tokens, long vocab, long padding,
   const long bytes = grad.numel() * grad.element_size();
   const int tiles = (int)ceil_div(n, kTile);
   const int clear = (int)std::min(1024L, std::max(1L, bytes / 16384));
-  auto counts = torch::empty({(long)kDigits * tiles}, keys.options());
+  auto counts = torch::empty({(long)kDigits * (tiles + 1)}, keys.options());
+  int* totals = counts.data_ptr<int>() + (long)kDigits * tiles;
   auto keys2 = torch::empty_like(keys);
   auto positions2 = torch::empty_like(positions);
   const int passes = (key_bits + 7) / 8;
@@ -726,14 +727,14 @@ void launch_big_sort(const torch::Tensor& tokens, long vocab, long padding,
                        counts.data_ptr<int>(),
                        static_cast<char*>(grad.data_ptr()), bytes);
     CHECK_HIP(hipGetLastError());
-    hipLaunchKernelGGL(scan_counts_kernel, dim3(1), dim3(1024), 0, stream,
-                       counts.data_ptr<int>(), kDigits * tiles);
+    hipLaunchKernelGGL(scan_counts_kernel, dim3(kDigits), dim3(kThreads), 0,
+                       stream, counts.data_ptr<int>(), tiles, totals);
     CHECK_HIP(hipGetLastError());
     auto* k = reinterpret_cast<uint32_t*>(keys2.data_ptr<int>());
     auto* p = reinterpret_cast<uint32_t*>(positions2.data_ptr<int>());
     hipLaunchKernelGGL(tile_scatter_kernel, dim3(tiles), dim3(kThreads), 0,
                        stream, in, n, tiles, pass * width, width,
-                       counts.data_ptr<int>(), k, p);
+                       counts.data_ptr<int>(), totals, k, p);
     CHECK_HIP(hipGetLastError());
     in.keys = k;
     in.positions = p;
