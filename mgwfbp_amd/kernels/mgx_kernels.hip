@@ -74,7 +74,9 @@ struct Chunk {
 // sgd_norm_partials_kernel left; every block adds them up in the same
 // order and folds min(1, max_norm / (norm + eps)) into grad_scale, so
 // clipping costs one read of the gradients and writes none of them. Block
-// 0 leaves the norm of the scaled gradients in norm_out.
+// 0 leaves the norm of the scaled gradients in norm_out. Measured, 66M
+// parameters without momentum: norm 40 us (6.6 TB/s), update 143 us (5.5
+// TB/s); clipping in place before it would read and write 528 MB more.
 //
 // PAST (with CLIP): every access goes past the 256 MB cache, for more than
 // it holds.
