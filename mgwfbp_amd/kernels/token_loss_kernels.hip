@@ -18,10 +18,10 @@
 // fused multiply-add, x log2 e - K, whose only rounding is that of the
 // result; K, the reference in these units, is held within +-kFar, where
 // that is exact enough, and nothing is tested for each element. A row
-// whose s does not come out positive and finite (a NaN, an infinity,
-// nothing but -inf, or logits beyond kFar, such as a row masked with the
-// type's lowest value) is done again by slow_row, which subtracts first
-// and takes every case; its stats are told apart by a negative s.
+// whose s does not come out sane (a NaN, an infinity, nothing but -inf, or
+// logits beyond kFar, such as a row masked with the type's lowest value) is
+// done again by slow_row, which subtracts first and takes every case; its
+// stats are told apart by a negative s.
 //
 // Measured: 8190 x 50001 bf16, loss and gradient 303 us, of which 285 (5.7
 // TB/s) in row_loss_kernel; 4095 x 32768 bf16, log probabilities with
@@ -177,7 +177,12 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ bool sane(float s) { return s > 0.f && s < kInf; }
+// Whether the fast way has given a sum to go on with: not 0, infinite or
+// NaN, and not so far from 1 that what is divided by it might lose bits
+// (the reference may be well below the maximum, see Held::guess).
+__device__ __forceinline__ bool sane(float s) {
+  return s > 1e-18f && s < 1e18f;
+}
 
 // Every case, by the whole block, from memory: the maximum, then sums of
 // what is left when it is subtracted. Returns s as it is stored; ref and u
@@ -219,7 +224,7 @@ __device__ __forceinline__ float slow_row(const T* x, int n, float* lds,
   }
   ref = m;
   u = v;
-  return sane(s) ? -s : __builtin_nanf("");
+  return s > 0.f && s < kInf ? -s : __builtin_nanf("");
 }
 
 // A stretch of a row as its vectors: whole ones that begin at multiples of
@@ -313,8 +318,9 @@ struct Held {
     return a;
   }
   // A reference for the thread's share: the maximum of its first vector, or
-  // of all where that one is masked. A value more than e^88 above it makes
-  // the sum infinite, and the row is done the slow way.
+  // of all where that one is masked. It serves for s alone; u would lose
+  // what the reference lacks of the maximum. Where all the block's guesses
+  // are more than 41 below the row's maximum, s is not sane any more.
   __device__ __forceinline__ float guess() const {
     const u32x4 q = vec(0);
     float m = -kInf;
@@ -648,8 +654,8 @@ __global__ __launch_bounds__(BLOCK, waves_for(NV, TOP)) void held_stats_kernel(
   const Target target = Target::of(x - from, row, w);
   Held<T, BLOCK, NV> held;
   held.load(x, n);
-  const float top = TOP ? held.max() : held.guess();
-  if (TOP) held.unpack_again();
+  const float top = held.max();
+  held.unpack_again();
   Stat a = held.template stat<true>(top);
   block_merge<true, BLOCK>(a, lds);
   const Row r = finish_slice<T, BLOCK>(x, target, a, row, part, w, out, lds,
@@ -723,7 +729,7 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(
 }
 
 // The loss of a row and its gradient, from one read: the row is held in
-// the block's registers, 32 to 64 of them for a thread, while its sums are
+// the block's registers, 4 to 64 of them for a thread, while its sums are
 // worked out. The gradient is that of the summed loss, times *share if
 // given, times one; what comes in for it in the backward pass is nearly
 // always that, and rescale_rows_kernel sees to the rest. Up to kCountHere
@@ -1084,7 +1090,8 @@ void launch_stats(const torch::Tensor& x, const torch::Tensor& targets,
   CHECK_HIP(hipGetLastError());
   if (splits > 1) {
     hipLaunchKernelGGL((join_rows_kernel<T, TOP>),
-                       grid_of(rows, kThreads, "rows"), dim3(kThreads), 0, stream, px, w, out, ps, pk);
+                       grid_of(rows, kThreads, "rows"), dim3(kThreads), 0,
+                       stream, px, w, out, ps, pk);
     CHECK_HIP(hipGetLastError());
   }
 }
@@ -1157,11 +1164,13 @@ torch::Tensor grad_of(const torch::Tensor& x, const GradIn& in,
     } else {
       const dim3 grid = grid_of(rows * parts, kThreads, "rows");
       if (in.grad_entropy != nullptr)
-        hipLaunchKernelGGL((row_grad_kernel<T, true>), grid, dim3(kThreads), 0, stream, px, (long)x.stride(0),
-                           vocab, (int)parts, slice, in, py);
+        hipLaunchKernelGGL((row_grad_kernel<T, true>), grid, dim3(kThreads),
+                           0, stream, px, (long)x.stride(0), vocab,
+                           (int)parts, slice, in, py);
       else
-        hipLaunchKernelGGL((row_grad_kernel<T, false>), grid, dim3(kThreads), 0, stream, px, (long)x.stride(0),
-                           vocab, (int)parts, slice, in, py);
+        hipLaunchKernelGGL((row_grad_kernel<T, false>), grid, dim3(kThreads),
+                           0, stream, px, (long)x.stride(0), vocab,
+                           (int)parts, slice, in, py);
     }
     CHECK_HIP(hipGetLastError());
   });

@@ -325,3 +325,42 @@ def test_together_a_language_model_step():
         assert torch.allclose(a, b, rtol=1e-4)
     for p, q in zip(sides[0][0].parameters(), sides[1][0].parameters()):
         assert torch.allclose(p, q, rtol=1e-3, atol=1e-5)
+
+
+def test_together_the_trainer():
+    """DLTrainer on the word-level model: the embedding, the loss and the
+    clipped update in training, the log probabilities in test()."""
+    from mgwfbp_amd.distributed_optimizer import DistributedOptimizer
+    from mgwfbp_amd.dl_trainer import DLTrainer
+    from mgwfbp_amd.kernels.token_loss import MgxCrossEntropyLoss
+    torch.manual_seed(0)
+    t = DLTrainer(0, 1, dist=False, batch_size=4, is_weak_scaling=True,
+                  ngpus=1, data_dir='', dataset='ptb', dnn='lstm', lr=1.0,
+                  nworkers=1, prefix='t', synthetic=True)
+    assert isinstance(t.net.embedding, em.MgxEmbedding)
+    assert isinstance(t.criterion, MgxCrossEntropyLoss)
+    opt = DistributedOptimizer(
+        t.optimizer, named_parameters=list(t.net.named_parameters()))
+    t.update_optimizer(opt)
+    before = [p.detach().clone() for p in t.net.parameters()]
+    hidden = t.net.init_hidden()
+    for _ in range(2):
+        opt.zero_grad()
+        _, hidden = t.train(1, hidden=hidden)
+        t.update_model(max_grad_norm=0.25)
+    moved = [p.detach() - b for p, b in zip(t.net.parameters(), before)]
+    assert all(torch.isfinite(m).all() for m in moved)
+    # two updates with lr 1 and gradients of norm at most 0.25 each
+    norm = sum(float(m.double().square().sum()) for m in moved) ** 0.5
+    assert 0.0 < norm <= 0.5 * (1 + 1e-4)
+    t.testloader = [b for b, _ in zip(t.testloader, range(2))]
+    ppl = t.test(0)
+    t.net.eval()
+    total = 0.0
+    with torch.no_grad():
+        for x, y in t.testloader:
+            out, _ = t.net(x.cuda(), t.net.init_hidden())
+            total += torch.nn.functional.cross_entropy(
+                out.view(-1, 10000), y.cuda().view(-1)).item()
+    assert abs(math.log(ppl) - total / 2) < 1e-4
+    assert 0.0 <= t.top5_accuracy <= 1.0 and t.mean_entropy > 0.0

@@ -259,6 +259,50 @@ def test_masks(vocab, kind):
     assert torch.isfinite(got).all() and bool((got[4] == 0).all())
 
 
+@pytest.mark.parametrize('kind', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('vocab', [2500, 10001, 50001])
+def test_peaks_and_offsets(vocab, kind):
+    """One logit far above the rest, rows far from zero, and rows whose
+    beginning is far below their end. A peaked row's entropy is small, and
+    right to a part of itself: H is at least what the peak's own term says."""
+    ups = [5.0, 15.0, 20.0, 30.0, 40.0, 42.0, 60.0, 88.0, 90.0, 120.0, 1e4]
+    offs = [-1e4, -300.0, -65.0, 65.0, 1e4, 3e6, -3e6, 1e30, -1e30]
+    x, t = _make(len(ups) + len(offs) + 3, vocab, kind, seed=18, scale=1.0)
+    for i, u in enumerate(ups):
+        x[i, vocab // 2 + i] += u
+        if i % 2:
+            t[i] = vocab // 2 + i
+    for i, o in enumerate(offs):
+        x[len(ups) + i] += o
+    x[-3, : vocab - 100] -= 1e4          # the usual finite masks
+    x[-2, : vocab // 2] -= 80.0
+    x[-1, ::2] -= 50.0
+    x.requires_grad_(True)
+    log, p, h = _exact(x)
+    r = tl.token_log_probs(x, t)
+    lp = log.gather(1, t[:, None])[:, 0]
+    # t is off by u |t| and log s by REL, and a product follows
+    far = REL + 4 * U * lp.abs()
+    assert bool(((r.log_probs.double() - lp).abs() <= far).all())
+    # u / s and log2 s are both near 0 in a peaked row: REL is of s - 1
+    assert bool(((r.entropy.double() - h).abs()
+                 <= 4 * REL * h + 16 * U).all()), \
+        ((r.entropy.double() - h).abs() / (4 * REL * h + 16 * U)).max()
+    rows = x.size(0)
+    hot = torch.zeros_like(p)
+    hot[torch.arange(rows), t] = 1.0
+    loss = tl.cross_entropy(x, t, reduction='sum')
+    want = -lp.sum()
+    assert abs(float(loss.detach()) - float(want)) <= \
+        rows * REL + 4 * U * float(lp.abs().sum())
+    got, = torch.autograd.grad(loss, x)
+    one = torch.ones_like(p)
+    _near_grad(got, p - hot, p, one, kind)
+    got, = torch.autograd.grad(
+        tl.cross_entropy(x, t, reduction='none').sum(), x)
+    _near_grad(got, p - hot, p, one, kind)
+
+
 @pytest.mark.parametrize('value', [float('nan'), float('inf')])
 def test_rows_that_are_not_finite(value):
     x, t = _make(3, 5000, torch.float32, seed=9)
