@@ -26,8 +26,7 @@
 // Measured: 8190 x 50001 bf16, loss and gradient 303 us, of which 285 (5.7
 // TB/s) in row_loss_kernel; 4095 x 32768 bf16, log probabilities with
 // entropy 47 us (5.7 TB/s) and their gradient 82 (6.5 TB/s); 700 x 10000
-// float32 with the best five 10 us; 4 x 50001 bf16 with the best eight, split
-// over 100 blocks, 6 us and 5 for the join.
+// float32 with the best five 10 us; 4 x 50001 bf16 with the best eight 9.
 //
 // A logit of -inf has p = 0 and adds nothing anywhere (t is held at kFloor
 // where it is a factor, so that no 0 * inf arises). A row with a NaN, a
@@ -560,11 +559,10 @@ __device__ __forceinline__ void put_best(const Row& r, const Where& w,
   }
 }
 
-// One block a row, or `splits` blocks a row that each leave what they
-// found of their slice for join_rows_kernel: with few rows one block
-// cannot draw the bandwidth of the card. This one takes slices too long
-// for held_stats_kernel: they stream past, and with TOP are read a second
-// time.
+// One block a row, or, for rows that one block cannot hold, `splits` of
+// them that each leave what they found of their slice for
+// join_rows_kernel. This one takes slices too long for held_stats_kernel:
+// they stream past, and with TOP are read a second time.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void row_stats_kernel(
     const T* __restrict__ logits, Where w, RowOut out,
@@ -634,14 +632,15 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(
 // Waves on each SIMD that a block of NV vectors a thread leaves registers
 // for: two blocks or more on a CU, so that one's loads run beside another's
 // arithmetic, but for the longest slices.
-constexpr int waves_for(int nv, bool top = false) {
-  return nv <= 4 ? 8 : nv <= 12 ? (top ? 5 : 6) : 4;
+constexpr int waves_for(int block, int nv, bool top = false) {
+  return nv <= 4 ? 8 : block == 1024 ? 4 : top ? 5 : 6;
 }
 
 // The same for a slice that fits the registers of a block: all its loads
 // are under way at once, and what comes after reads no memory.
 template <typename T, int BLOCK, int NV, bool TOP>
-__global__ __launch_bounds__(BLOCK, waves_for(NV, TOP)) void held_stats_kernel(
+__global__ __launch_bounds__(
+    BLOCK, waves_for(BLOCK, NV, TOP)) void held_stats_kernel(
     const T* __restrict__ logits, Where w, RowOut out,
     float* __restrict__ part_stats, uint64_t* __restrict__ part_keys) {
   __shared__ float lds[3 * BLOCK / 64];
@@ -738,7 +737,7 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(
 constexpr int kCountHere = 1024;
 
 template <typename T, int BLOCK, int NV>
-__global__ __launch_bounds__(BLOCK, waves_for(NV)) void row_loss_kernel(
+__global__ __launch_bounds__(BLOCK, waves_for(BLOCK, NV)) void row_loss_kernel(
     const T* __restrict__ logits, Where w, RowOut out, long rows, bool mean,
     const float* __restrict__ share, T* __restrict__ grad) {
   constexpr int V = Elem<T>::kVec;
@@ -1004,14 +1003,20 @@ void check_inputs(const torch::Tensor& logits, const torch::Tensor& targets) {
 
 // A block and its registers for `vecs` vectors of a row or of a slice: the
 // smallest that holds them; f gets BLOCK and NV as constants. False if none
-// does. A slice takes two blocks on a CU at least (kHeldSlice vectors); a
-// whole row, which cannot be split where its gradient leaves with it, twice
-// that and more.
+// does.
+//
+// With many blocks a slice is one that leaves room for a second on the CU;
+// with no more of them than CUs it is twice that, since a second launch to
+// join slices costs more than it gives: best eight of 4 x 50001 bf16 10.2 us
+// against 12.1 by 25 slices, 4 x 20000 float32 8.5 against 12.0; but 1024 x
+// 20000 float32 32.6 against 24.0 us, 256 x 131072 41.9 against 31.8.
+constexpr long kFewBlocks = 256;
 constexpr long kHeldSlice = 4096;
+constexpr long kHeldFew = 8192;
 constexpr long kHeldLeast = 16;   // elements: a whole vector for certain
 
 template <typename F>
-bool with_slice(long vecs, F&& f) {
+bool with_slice(long vecs, bool few, F&& f) {
   using std::integral_constant;
   if (vecs <= 256)
     f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
@@ -1023,15 +1028,18 @@ bool with_slice(long vecs, F&& f) {
     f(integral_constant<int, 512>{}, integral_constant<int, 5>{});
   else if (vecs <= kHeldSlice)
     f(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+  else if (few && vecs <= kHeldFew)
+    f(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
   else
     return false;
   return true;
 }
 
+// A whole row, which cannot be split where its gradient leaves with it.
 template <typename F>
 bool with_row(long vecs, F&& f) {
   using std::integral_constant;
-  if (with_slice(vecs, f)) return true;
+  if (vecs <= kHeldSlice) return with_slice(vecs, false, f);
   if (vecs <= 9216)
     f(integral_constant<int, 768>{}, integral_constant<int, 12>{});
   else if (vecs <= 16384)
@@ -1053,13 +1061,11 @@ void launch_stats(const torch::Tensor& x, const torch::Tensor& targets,
   const long rows = x.size(0);
   const int vocab = (int)x.size(1);
   const int step = kThreads * Elem<T>::kVec;
-  // Blocks enough for the card, and a slice that is worth a block, but no
-  // longer than one holds.
-  const long least = TOP ? step : 4L * step;
+  const bool few =
+      rows * ceil_div(vocab, kHeldFew * Elem<T>::kVec) <= kFewBlocks;
   const long most = TOP ? std::min(kJoin / k, kMaxSplits) : kMaxSplits;
-  long splits = std::min(ceil_div(512, rows), ceil_div(vocab, least));
-  splits = std::max(splits, ceil_div(vocab, kHeldSlice * Elem<T>::kVec));
-  splits = std::max(std::min(splits, most), 1L);
+  long splits = std::min(
+      ceil_div(vocab, (few ? kHeldFew : kHeldSlice) * Elem<T>::kVec), most);
   Where w = where(x, targets, ignore, k);
   if (splits > 1)
     w.slice = (int)(ceil_div(ceil_div(vocab, splits), step) * step);
@@ -1078,7 +1084,7 @@ void launch_stats(const torch::Tensor& x, const torch::Tensor& targets,
       ? reinterpret_cast<uint64_t*>(keys.data_ptr<int64_t>()) : nullptr;
   const T* px = static_cast<const T*>(x.data_ptr());
   const bool held = vocab >= kHeldLeast &&
-      with_slice(w.slice / Elem<T>::kVec, [&](auto block, auto nv) {
+      with_slice(w.slice / Elem<T>::kVec, few, [&](auto block, auto nv) {
         hipLaunchKernelGGL((held_stats_kernel<T, block.value, nv.value, TOP>),
                            grid_of(rows * splits, block.value, "rows"),
                            dim3(block.value), 0, stream, px, w, out, ps, pk);
