@@ -17,7 +17,7 @@ torch::Tensor embedding(const torch::Tensor& tokens,
                         int64_t padding);
 torch::Tensor cross_entropy(const torch::Tensor& logits,
                             const torch::Tensor& targets, int64_t ignore,
-                            int64_t reduction);
+                            int64_t reduction, bool scaled);
 std::vector<torch::Tensor> token_log_probs(const torch::Tensor& logits,
                                            const torch::Tensor& targets,
                                            int64_t k, int64_t ignore);

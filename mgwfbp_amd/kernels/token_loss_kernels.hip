@@ -713,7 +713,7 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(
     float* __restrict__ share) {
   __shared__ int waves[16];
   int c = 0;
-#pragma unroll 8
+#pragma unroll 4
   for (long i = threadIdx.x; i < rows; i += 1024)
     c += target_at(targets, wide, i) != ignore;
 #pragma unroll
@@ -822,7 +822,7 @@ __global__ __launch_bounds__(1024) void reduce_loss_kernel(
   __shared__ double sums[16];
   __shared__ double kept[16];
   double s = 0., c = 0.;
-#pragma unroll 8
+#pragma unroll 4
   for (long i = threadIdx.x; i < rows; i += 1024) {
     s += each[i];
     c += target_at(targets, wide, i) != ignore ? 1. : 0.;
@@ -1157,7 +1157,9 @@ torch::Tensor grad_of(const torch::Tensor& x, const GradIn& in,
   const int vocab = (int)x.size(1);
   with_elem(x.scalar_type(), "logits", [&](auto z) {
     using T = decltype(z);
-    const int slice = 4 * kThreads * Elem<T>::kVec;
+    // blocks that stay take longer slices: what comes before a slice's first
+    // load is a latency of its own
+    const int slice = (ready.defined() ? 32 : 4) * kThreads * Elem<T>::kVec;
     const long parts = ceil_div(vocab, slice);
     const T* px = static_cast<const T*>(x.data_ptr());
     T* py = static_cast<T*>(out.data_ptr());
@@ -1328,7 +1330,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
 
 torch::Tensor cross_entropy(const torch::Tensor& logits,
                             const torch::Tensor& targets, int64_t ignore,
-                            int64_t reduction) {
+                            int64_t reduction, bool scaled) {
   check_inputs(logits, targets);
   TORCH_CHECK_VALUE(reduction >= kNone && reduction <= kSum,
                     "unknown reduction ", reduction);
@@ -1336,7 +1338,7 @@ torch::Tensor cross_entropy(const torch::Tensor& logits,
   c10::DeviceGuard guard(logits.device());
   auto loss = CrossEntropy::apply(
       as_rows(logits), targets.reshape({-1}).contiguous(), ignore, reduction,
-      at::GradMode::is_enabled() && logits.requires_grad());
+      !scaled && at::GradMode::is_enabled() && logits.requires_grad());
   return reduction == kNone && targets.dim() != 1
       ? loss.view(targets.sizes()) : loss;
 }

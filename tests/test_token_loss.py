@@ -82,7 +82,7 @@ def test_native_entries_refuse_host_tensors():
     ext = load_lm()
     x, t = torch.randn(3, 5), torch.tensor([0, 1, 2])
     with pytest.raises(ValueError):
-        ext.cross_entropy(x, t, -100, 1)
+        ext.cross_entropy(x, t, -100, 1, False)
     with pytest.raises(ValueError):
         ext.token_log_probs(x, t, 0, -100)
 

@@ -160,9 +160,11 @@ def test_loss_scaled_afterwards(kind, scale):
     log, p, _ = _exact(x)
     hot = torch.zeros_like(p)
     hot[torch.arange(37), t] = 1.0
-    got, = torch.autograd.grad(tl.cross_entropy(x, t) * scale, x)
-    _near_grad(got, (p - hot) * scale / 37, p,
-               torch.full_like(p, scale / 37), kind)
+    for told in (False, True):
+        loss = tl.cross_entropy(x, t, scaled=told) * scale
+        got, = torch.autograd.grad(loss, x)
+        _near_grad(got, (p - hot) * scale / 37, p,
+                   torch.full_like(p, scale / 37), kind)
 
 
 def test_backward_twice_and_after():
