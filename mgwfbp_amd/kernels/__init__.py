@@ -8,6 +8,9 @@ snapshot to GPU boxes:
   pack/unpack(+cast/scale), L2 norm — the gfx950 hot-path kernels.
 - ``mgx_comm_ext``     (mgwfbp_amd/comm/comm_core.hip): RCCL comm core.
 
+``mgx_bn_ext`` (batchnorm.py, pooling.py) and ``mgx_lm_ext`` (embedding.py,
+token_loss.py, grad_clip.py) are loaded by the modules that use them.
+
 Policy: on a GPU box the HIP path MUST run — ops raise loudly if the
 extension is missing while CUDA is available (no silent eager fallback).
 On CPU (the test tier) pure-torch reference implementations are used; the
