@@ -308,6 +308,11 @@ class DLTrainer:
                                          rank=self.rank)
         self.train_sampler = sampler
         collate = mgx_data.an4_collate if self.dataset == 'an4' else None
+        # The word-level text lies in memory, and a batch is a slice of it:
+        # no worker processes, which would be forked from one that may hold
+        # a GPU.
+        train_workers, test_workers = \
+            (0, 0) if self.dataset == 'ptb' else (2, 1)
         if self.dataset == 'an4' and self.nworkers > 1:
             batch_sampler = mgx_data.DistributedBucketingSampler(
                 ds, batch_size=self.batch_size,
@@ -320,11 +325,12 @@ class DLTrainer:
             self.trainloader = DataLoader(
                 ds, batch_size=self.batch_size,
                 shuffle=(sampler is None), sampler=sampler,
-                collate_fn=collate, num_workers=2, drop_last=True)
+                collate_fn=collate, num_workers=train_workers,
+                drop_last=True)
         self.testloader = DataLoader(self.testset,
                                      batch_size=self.batch_size,
                                      shuffle=False, collate_fn=collate,
-                                     num_workers=1)
+                                     num_workers=test_workers)
         self.num_batches_per_epoch = max(
             len(self.trainset) // (self.batch_size * max(self.nworkers, 1)),
             1)
