@@ -7,6 +7,14 @@
 //   log p_j = ln 2 (t_j - log2 s)        entropy H = ln 2 (log2 s - u / s)
 //   d log p_t / d x_j = [j = t] - p_j    d H / d x_j = -p_j (log p_j + H)
 //
+// The reference has to be near for the differences' sake: one that is d
+// binary orders below the maximum leaves both sides of them near d, and a
+// log probability or an entropy near 0 is then off by d roundings. So it is
+// the maximum of what is held or has streamed past so far; only the loss,
+// which needs no u, takes one from a part of the row and the target, see
+// row_loss_kernel. What the last rounding leaves on the wrong side of 0 is
+// set to 0.
+//
 // All of it is bound by memory: a row is read once for s and u (in 32
 // bits), and a gradient is one more read and a write. Where the loss is to
 // be differentiated its gradient leaves the forward pass, from a row that
@@ -89,26 +97,18 @@ struct Stat {
     s += e;
     if (ENT) u = fmaf(e, fmaxf(t, kFloor), u);
   }
-  // Elements whose maximum is not known: they are taken against the
-  // reference at hand, and once more if that was too low for them.
+  // N more elements, whose maximum is the result: the reference is raised
+  // to it first where it is lower.
   template <int N, typename F>
-  __device__ __forceinline__ void add_all(F&& x) {
-    Stat c;
-    c.k = k;
+  __device__ __forceinline__ float add_all(F&& x) {
+    float m = -kInf;
 #pragma unroll
-    for (int i = 0; i < N; ++i) c.template add<true>(x(i));
-    if (!(c.s < 1e30f)) {
-      float m = -kInf;
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x(i));
+    const float to = ref(m);
+    if (to > k) raise(to);
 #pragma unroll
-      for (int i = 0; i < N; ++i) m = fmaxf(m, x(i));
-      raise(fmaxf(k, ref(m)));
-      c = Stat();
-      c.k = k;
-#pragma unroll
-      for (int i = 0; i < N; ++i) c.template add<true>(x(i));
-    }
-    s += c.s;
-    u += c.u;
+    for (int i = 0; i < N; ++i) add<true>(x(i));
+    return m;
   }
 };
 
@@ -168,19 +168,24 @@ struct Row {
   __device__ __forceinline__ float t(float x) const {
     return SLOW ? (x - ref) * kLog2e : fmaf(x, kLog2e, -ref);
   }
+  // a NaN stays one
   __device__ __forceinline__ float log_prob(float x) const {
-    return kLn2 * ((slow ? t<true>(x) : t<false>(x)) - log2s);
+    const float lp = kLn2 * ((slow ? t<true>(x) : t<false>(x)) - log2s);
+    return lp > 0.f ? 0.f : lp;
   }
   __device__ __forceinline__ float entropy(float u) const {
-    return kLn2 * (log2s - u / s);
+    const float h = kLn2 * (log2s - u / s);
+    return h < 0.f ? 0.f : h;
   }
 };
 
-// Whether the fast way has given a sum to go on with: not 0, infinite or
-// NaN, and not so far from 1 that what is divided by it might lose bits
-// (the reference may be well below the maximum, see Held::guess).
-__device__ __forceinline__ bool sane(float s) {
-  return s > 1e-18f && s < 1e18f;
+// Whether the fast way has given a sum to go on with. Against its maximum,
+// or kLower below, a row of n logits has one between 1 and n, or 2^kLower
+// times that; not so where the reference was held at +-kFar, or where
+// something is not finite.
+constexpr float kLower = 10.f;
+__device__ __forceinline__ bool sane(float s, int n) {
+  return s > 0.25f && s < 2048.f * (float)n;
 }
 
 // Every case, by the whole block, from memory: the maximum, then sums of
@@ -317,9 +322,8 @@ struct Held {
     return a;
   }
   // A reference for the thread's share: the maximum of its first vector, or
-  // of all where that one is masked. It serves for s alone; u would lose
-  // what the reference lacks of the maximum. Where all the block's guesses
-  // are more than 41 below the row's maximum, s is not sane any more.
+  // of all where that one is masked. It serves for s alone, and where it
+  // turns out to be no more than kLower below the row's maximum.
   __device__ __forceinline__ float guess() const {
     const u32x4 q = vec(0);
     float m = -kInf;
@@ -517,6 +521,22 @@ struct Target {
     t.x = Elem<T>::up(row_x[t.id >= 0 && t.id < w.vocab ? t.id : 0]);
     return t;
   }
+  // The same where the block takes the row whole, as a scalar load of the
+  // word that the logit lies in: what waits for it need not wait for the
+  // row, as it would behind vector loads, which come back in order.
+  template <typename T>
+  static __device__ __forceinline__ Target of_row(const T* row_x, long row,
+                                                  const Where& w) {
+    typedef const __attribute__((address_space(4))) uint32_t* Word;
+    Target t;
+    t.id = target_at(w.targets, w.wide, row);
+    const auto at = reinterpret_cast<uintptr_t>(
+        row_x + (t.id >= 0 && t.id < w.vocab ? t.id : 0));
+    const uint32_t word = *(Word)(at & ~(uintptr_t)3);
+    t.x = Elem<T>::get(u32x4{word, 0u, 0u, 0u},
+                       (int)(at & 3) / (int)sizeof(T));
+    return t;
+  }
 };
 
 // What a block found of its slice: the row's outputs where it is the whole
@@ -536,7 +556,7 @@ __device__ __forceinline__ Row finish_slice(const T* x, const Target& t,
     }
     return Row(0.f, 1.f);
   }
-  if (!sane(s)) s = slow_row<T, BLOCK>(x, w.vocab, lds, ref, u);
+  if (!sane(s, w.vocab)) s = slow_row<T, BLOCK>(x, w.vocab, lds, ref, u);
   const Row r(ref, s);
   if (threadIdx.x == 0)
     finish_row(r, u, row, w.vocab, t.x, t.id, w.ignore, out);
@@ -590,25 +610,16 @@ __global__ __launch_bounds__(kThreads) void row_stats_kernel(
     for (int q = 0; q < U; ++q)
       r[q] = load16_past(xv + (i + q * kThreads) * V);
     const auto get = [&](int e) { return Elem<T>::get(r[e / V], e % V); };
-    a.template add_all<U * V>(get);
-    if (TOP) {
-#pragma unroll
-      for (int e = 0; e < U * V; ++e) top = fmaxf(top, get(e));
-    }
+    top = fmaxf(top, a.template add_all<U * V>(get));
   }
   for (; i < p.vecs; i += kThreads) {
     const u32x4 r = load16_past(xv + i * V);
     const auto get = [&](int e) { return Elem<T>::get(r, e); };
-    a.template add_all<V>(get);
-    if (TOP) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = fmaxf(top, get(e));
-    }
+    top = fmaxf(top, a.template add_all<V>(get));
   }
   if (tid < p.edges) {
     const float v = Elem<T>::up(x[p.edge<V>(tid)]);
-    a.template add_all<1>([&](int) { return v; });
-    if (TOP) top = fmaxf(top, v);
+    top = fmaxf(top, a.template add_all<1>([&](int) { return v; }));
   }
   block_merge<true, kThreads>(a, lds);
   const Row r =
@@ -734,6 +745,12 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(
 // always that, and rescale_rows_kernel sees to the rest. Up to kCountHere
 // rows the block counts the rows that are kept itself, which costs less
 // than a launch.
+//
+// The reference is the maximum of the threads' first vectors, so that the
+// exponentials begin when those have come, and of the target, beside which
+// the loss may be small. A logit that is far above both shows in s: then
+// the row's maximum is looked for, and if it is more than kLower above, the
+// sums are taken once more, from the registers.
 constexpr int kCountHere = 1024;
 
 template <typename T, int BLOCK, int NV>
@@ -747,9 +764,9 @@ __global__ __launch_bounds__(BLOCK, waves_for(BLOCK, NV)) void row_loss_kernel(
   const long row = blockIdx.x;
   const int n = w.vocab;
   const T* __restrict__ x = logits + row * w.row_stride;
+  const Target target = Target::of_row(x, row, w);
   Held<T, BLOCK, NV> held;
   held.load(x, n);
-  const Target target = Target::of(x, row, w);
   int c = 0;
   if (mean && share == nullptr) {
     for (int i = threadIdx.x; i < (int)rows; i += BLOCK)
@@ -758,8 +775,17 @@ __global__ __launch_bounds__(BLOCK, waves_for(BLOCK, NV)) void row_loss_kernel(
     for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
     if ((threadIdx.x & 63) == 0) kept[threadIdx.x >> 6] = c;
   }
-  Stat a = held.template stat<false>(held.guess());
+  Stat a = held.template stat<false>(fmaxf(held.guess(), target.x));
   block_merge<false, BLOCK>(a, lds);    // a barrier: kept is there too
+  if (!(a.s <= 1024.f)) {               // 2^kLower
+    held.unpack_again();
+    const float top = held.max();
+    if (__syncthreads_or(Stat::ref(top) > a.k + kLower)) {
+      held.unpack_again();
+      a = held.template stat<false>(top);
+      block_merge<false, BLOCK>(a, lds);
+    }
+  }
   float by = 1.f;
   if (mean) {
     if (share != nullptr) {

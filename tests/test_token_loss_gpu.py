@@ -571,3 +571,76 @@ def test_same_bits_every_time():
         if first is None:
             first = (loss, g)
         assert torch.equal(loss, first[0]) and torch.equal(g, first[1])
+
+
+def _bounds(log):
+    """How far a row's sum s may be off, relative, and M, the mean distance
+    from the maximum. Each term of s is off by 4 u and by 2 u of its distance
+    from the maximum, and on its way into s it is rounded at most A times: a
+    thread adds up at most 256 elements here, and twelve steps of the merges
+    take four roundings each. Roundings of a sum with the largest term in it
+    are no larger than what is added to it, so for a row with all but q of
+    its mass in one class they come to q at most."""
+    a = 320
+    p = log.exp()
+    best = log.amax(1)
+    q = (1.0 - best.exp()).clamp(min=0.0)
+    far = torch.minimum(a * U * torch.ones_like(q), q) + a * U * q + 8 * U
+    m = -(p * (log - best[:, None]).masked_fill(log == NEG, 0.0)).sum(1)
+    return far, m, a
+
+
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('vocab', [2, 5, 9, 15, 16, 300, 2500, 10001, 50001,
+                                   100003, 400003, 2100001])
+def test_statistics_of_peaked_rows(vocab, kind):
+    """A class far above the rest, wherever it stands, as the target and not:
+    the log probability is 0 at most, the entropy 0 at least, and both, the
+    loss and its gradient, are right to a few roundings of their own size,
+    which they are only if the sums are taken against a reference near the
+    row's maximum (beside one that is 20 below it, 30 u of a loss near 0 are
+    lost). t is within 2 u of itself and log2 s within 2, and a difference
+    follows: 6 u of the log probability."""
+    ups = [0.0, 0.5, 3.0, 9.0, 16.3, 21.0, 26.0, 30.0, 39.0, 50.0, 88.0]
+    places = [vocab - 1, vocab // 2, vocab // 3]
+    if vocab > 200000:
+        ups, places = ups[4:8], places[:2]
+    x, t = _make(len(ups) * len(places), vocab, kind, seed=30, scale=0.5)
+    for i, u in enumerate(ups):
+        for j, at in enumerate(places):
+            row = i * len(places) + j
+            x[row, at] = u + 1.0
+            t[row] = at if (i + j) % 3 else 1
+    x.requires_grad_(True)
+    r = tl.token_log_probs(x.detach(), t, top_k=1)
+    each = tl.cross_entropy(x, t, reduction='none').detach()
+    for i in range(x.size(0)):
+        log, p, h = _exact(x[i:i + 1])
+        far, m, a = _bounds(log)
+        far, m, h = float(far), float(m), float(h)
+        lp = float(log[0, t[i]])
+        near = far + 6 * U * abs(lp)
+        assert float(r.log_probs[i]) <= 0.0
+        assert abs(float(r.log_probs[i]) - lp) <= near, (i, lp)
+        assert float(r.top_log_probs[i, 0]) <= 0.0
+        top = float(log.max())
+        assert abs(float(r.top_log_probs[i, 0]) - top) <= \
+            far + 6 * U * abs(top)
+        assert float(r.entropy[i]) >= 0.0
+        assert abs(float(r.entropy[i]) - h) <= \
+            far + 8 * U * h + (a + 16) * U * m, (i, h)
+        y = x.detach()[i:i + 1].requires_grad_(True)
+        loss = tl.cross_entropy(y, t[i:i + 1])
+        for got in (float(loss.detach()), float(each[i])):
+            assert got >= 0.0
+            assert abs(got + lp) <= near, (i, got, -lp)
+        got, = torch.autograd.grad(loss, y)
+        # p is off as s is, and by 2 u of its exponent: its distance from the
+        # maximum, or from a reference up to 11 binary orders below that
+        want = p.clone()
+        want[0, t[i]] -= 1.0
+        off = (far + (16 + 2 * 11) * U) * p + 2 * U * p * log.abs().clamp(
+            max=1e4) + (torch.finfo(kind).eps / 2 + 2 * U) * want.abs() + \
+            {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126,
+             torch.float16: 2.0 ** -24}[kind]
+        assert bool(((got.double() - want).abs() <= off).all()), i
