@@ -183,9 +183,9 @@ struct Row {
 // or kLower below, a row of n logits has one between 1 and n, or 2^kLower
 // times that; not so where the reference was held at +-kFar, or where
 // something is not finite.
-constexpr float kLower = 10.f;
+constexpr float kLower = 17.f;
 __device__ __forceinline__ bool sane(float s, int n) {
-  return s > 0.25f && s < 2048.f * (float)n;
+  return s > 0.25f && s < 262144.f * (float)n;
 }
 
 // Every case, by the whole block, from memory: the maximum, then sums of
@@ -750,7 +750,12 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(
 // exponentials begin when those have come, and of the target, beside which
 // the loss may be small. A logit that is far above both shows in s: then
 // the row's maximum is looked for, and if it is more than kLower above, the
-// sums are taken once more, from the registers.
+// sums are taken once more, from the registers. 2^kLower is as many classes
+// as a row here has, so that an even row need not be looked through:
+// 8190 x 50001 bf16 nearly even logits take 310 us like others, and 348
+// with a kLower of 10. (All rows with a logit of 30 in the last place, not
+// the target: 353.) An exponent of 17 is off by 2^-20 at most, and so far
+// from the others' is then the probability of such a logit.
 constexpr int kCountHere = 1024;
 
 template <typename T, int BLOCK, int NV>
@@ -777,7 +782,7 @@ __global__ __launch_bounds__(BLOCK, waves_for(BLOCK, NV)) void row_loss_kernel(
   }
   Stat a = held.template stat<false>(fmaxf(held.guess(), target.x));
   block_merge<false, BLOCK>(a, lds);    // a barrier: kept is there too
-  if (!(a.s <= 1024.f)) {               // 2^kLower
+  if (!(a.s <= 131072.f)) {             // 2^kLower
     held.unpack_again();
     const float top = held.max();
     if (__syncthreads_or(Stat::ref(top) > a.k + kLower)) {
