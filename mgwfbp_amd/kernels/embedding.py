@@ -11,7 +11,8 @@ once, so a repeated call gives the same bits.
 The weight is float32, bfloat16 or float16; its gradient is dense and of
 its type. A token outside the table is an IndexError on the CPU; on a GPU,
 where finding it would take a synchronisation, nothing is read for it, its
-output is NaN and it has no gradient. There is no second derivative.
+output is NaN and it has no gradient. The function has no second derivative;
+the module has.
 """
 from __future__ import annotations
 
@@ -20,9 +21,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import settings
-from .grad_clip import load_lm
+from .grad_clip import load_lm, seen_whole
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_TOKENS = (torch.int64, torch.int32)
 
 
 def embedding(tokens, weight, scale=1.0, padding_idx=None):
@@ -39,7 +41,7 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
         return load_lm().embedding(tokens, weight, float(scale),
                                    -1 if padding_idx is None
                                    else padding_idx)
-    if tokens.dtype not in (torch.int64, torch.int32):
+    if tokens.dtype not in _TOKENS:
         raise TypeError('tokens must be int64 or int32, not %s'
                         % tokens.dtype)
     if tokens.device != weight.device:
@@ -50,27 +52,31 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
 
 
 class MgxEmbedding(nn.Embedding):
-    """nn.Embedding on the HIP kernels, with a factor on its output. The
-    options that only torch has (max_norm, sparse gradients, scaling by
-    frequency) and other types go to torch."""
+    """nn.Embedding on the HIP kernels, with a factor on its output, and
+    with second and further derivatives. The options that only torch has
+    (max_norm, sparse gradients, scaling by frequency), other types, and
+    calls that torch has to see as its own operations (torch.compile and
+    tracing, torch.func, forward-mode differentiation) go to torch."""
 
     def __init__(self, *args, scale=1.0, **kwargs):
         super().__init__(*args, **kwargs)
         self.scale = scale
 
-    def _use_hip_path(self, x):
-        return (settings.USE_HIP_KERNELS and self.weight.is_cuda
-                and x.device == self.weight.device
-                and x.dtype in (torch.int64, torch.int32)
-                and self.weight.dtype in _TYPES and self.max_norm is None
+    def _use_hip_path(self, x, w):
+        return (settings.USE_HIP_KERNELS and w.is_cuda
+                and x.device == w.device and seen_whole(x, w)
+                and x.dtype in _TOKENS and w.dtype in _TYPES
+                and self.max_norm is None
                 and not self.sparse and not self.scale_grad_by_freq)
 
     def forward(self, x):
-        if not self._use_hip_path(x):
+        w = self.weight
+        if not self._use_hip_path(x, w):
             y = super().forward(x)
             return y if self.scale == 1.0 else y * self.scale
-        return embedding(x, self.weight, scale=self.scale,
-                         padding_idx=self.padding_idx)
+        pad = self.padding_idx
+        return load_lm().embedding(x, w, float(self.scale),
+                                   -1 if pad is None else pad, True)
 
     def extra_repr(self):
         s = super().extra_repr()

@@ -36,6 +36,7 @@
 #include "lm_common.h"
 
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <vector>
@@ -837,40 +838,84 @@ torch::Tensor weight_grad(const torch::Tensor& tokens,
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+torch::Tensor grad_rows(const torch::Tensor& tokens, torch::Tensor dout,
+                        int64_t vocab, double scale, int64_t padding) {
+  c10::DeviceGuard guard(tokens.device());
+  if (dout.size(1) > 1 && dout.stride(1) != 1) dout = dout.contiguous();
+  return weight_grad(tokens, dout, vocab, dout.size(1), (float)scale,
+                     padding);
+}
+
+// `twice`: the backward pass may itself be differentiated. The rows' sums
+// are linear in dout, and their own gradient is a gather again, of zeros
+// for tokens that have no gradient.
 struct Embedding : torch::autograd::Function<Embedding> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor weight,
                                torch::Tensor tokens, double scale,
-                               int64_t padding) {
+                               int64_t padding, bool twice) {
     c10::DeviceGuard guard(weight.device());
     ctx->save_for_backward({tokens});
     ctx->saved_data["vocab"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
+    ctx->saved_data["twice"] = twice;
     return gather_rows(weight, tokens, (float)scale);
   }
+  static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
 
+struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor dout,
+                               torch::Tensor tokens, int64_t vocab,
+                               double scale, int64_t padding) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = vocab;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return grad_rows(tokens, dout, vocab, scale, padding);
+  }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(),
-                "the embedding has no second derivative: it cannot be "
-                "differentiated with create_graph=True");
     const auto tokens = ctx->get_saved_variables()[0];
-    c10::DeviceGuard guard(tokens.device());
-    auto dout = grads[0];
-    if (dout.size(1) > 1 && dout.stride(1) != 1) dout = dout.contiguous();
-    return {weight_grad(tokens, dout, ctx->saved_data["vocab"].toInt(),
-                        dout.size(1),
-                        (float)ctx->saved_data["scale"].toDouble(),
-                        ctx->saved_data["padding"].toInt()),
+    const int64_t padding = ctx->saved_data["padding"].toInt();
+    const auto g = grads[0].size(1) < 2 || grads[0].stride(1) == 1
+        ? grads[0] : grads[0].contiguous();
+    const auto out = Embedding::apply(
+        g, tokens, ctx->saved_data["scale"].toDouble(), padding, true);
+    const auto none = tokens.eq(padding)
+                          .logical_or(tokens.lt(0))
+                          .logical_or(
+                              tokens.ge(ctx->saved_data["vocab"].toInt()));
+    return {out.masked_fill(none.unsqueeze(1), 0), torch::Tensor(),
             torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
 };
+
+variable_list Embedding::backward(AutogradContext* ctx, variable_list grads) {
+  const auto tokens = ctx->get_saved_variables()[0];
+  const int64_t vocab = ctx->saved_data["vocab"].toInt();
+  const double scale = ctx->saved_data["scale"].toDouble();
+  const int64_t padding = ctx->saved_data["padding"].toInt();
+  torch::Tensor grad;
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK(ctx->saved_data["twice"].toBool(),
+                "the embedding has no second derivative: it cannot be "
+                "differentiated with create_graph=True");
+    grad = EmbeddingGrad::apply(grads[0], tokens, vocab, scale, padding);
+  } else {
+    grad = grad_rows(tokens, grads[0], vocab, scale, padding);
+  }
+  return {grad, torch::Tensor(), torch::Tensor(), torch::Tensor(),
+          torch::Tensor()};
+}
 
 }  // namespace
 
 // padding: a row that gets no gradient, or -1.
 torch::Tensor embedding(const torch::Tensor& tokens,
                         const torch::Tensor& weight, double scale,
-                        int64_t padding) {
+                        int64_t padding, bool twice) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(),
+              "the embedding kernel cannot be traced");
   TORCH_CHECK_VALUE(weight.is_cuda() && weight.dim() == 2,
                     "the embedding weight must be a matrix on a GPU");
   TORCH_CHECK_VALUE(weight.size(0) < (1L << 31) - 1 &&
@@ -890,7 +935,7 @@ torch::Tensor embedding(const torch::Tensor& tokens,
   const auto w = weight.size(1) < 2 || weight.stride(1) == 1
       ? weight : weight.contiguous();
   auto out = Embedding::apply(w, tokens.reshape({-1}).contiguous(), scale,
-                              padding);
+                              padding, twice);
   if (tokens.dim() == 1) return out;
   auto shape = tokens.sizes().vec();
   shape.push_back(weight.size(1));

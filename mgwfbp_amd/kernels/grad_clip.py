@@ -19,8 +19,14 @@ from __future__ import annotations
 import importlib
 
 import torch
+from torch.autograd import forward_ad
+from torch.compiler import is_compiling
 
 _ext = None
+_DATA = (torch.Tensor, torch.nn.Parameter)
+_tracing = torch._C._get_tracing_state
+_transforms = torch._C._are_functorch_transforms_active
+_modes = torch._C._len_torch_dispatch_stack
 
 
 def load_lm():
@@ -37,6 +43,17 @@ def load_lm():
                 'in-tree: python setup.py build_ext --inplace (original '
                 'error: %s)' % e)
     return _ext
+
+
+def seen_whole(x, y):
+    """Whether the tensors are data that a kernel can be given, with nothing
+    beside it that looks at the operations: no compiler or tracer, no
+    transform of torch.func, no forward-mode differentiation, no dispatch
+    mode, no tensor of another class. What stands for one of torch's modules
+    leaves those to torch's own operations."""
+    return not (is_compiling() or _tracing() is not None or _transforms()
+                or _modes() or forward_ad._current_level >= 0) and \
+        type(x) in _DATA and type(y) in _DATA
 
 
 def _limits(max_norm, eps):

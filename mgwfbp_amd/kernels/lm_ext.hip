@@ -14,10 +14,10 @@ torch::Tensor clip_grads_(const std::vector<torch::Tensor>& grads,
 
 torch::Tensor embedding(const torch::Tensor& tokens,
                         const torch::Tensor& weight, double scale,
-                        int64_t padding);
+                        int64_t padding, bool twice);
 torch::Tensor cross_entropy(const torch::Tensor& logits,
                             const torch::Tensor& targets, int64_t ignore,
-                            int64_t reduction, bool scaled);
+                            int64_t reduction, bool scaled, bool twice);
 std::vector<torch::Tensor> token_log_probs(const torch::Tensor& logits,
                                            const torch::Tensor& targets,
                                            int64_t k, int64_t ignore);
@@ -31,9 +31,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("clip_grads_", &mgx::clip_grads_,
         "Scale gradients in place to a global norm; returns the norm");
   m.def("embedding", &mgx::embedding,
-        "Rows of a table by token, scaled (differentiable)");
+        "Rows of a table by token, scaled (differentiable)",
+        py::arg("tokens"), py::arg("weight"), py::arg("scale"),
+        py::arg("padding"), py::arg("twice") = false);
   m.def("cross_entropy", &mgx::cross_entropy,
-        "Cross entropy of logits and class indices (differentiable)");
+        "Cross entropy of logits and class indices (differentiable)",
+        py::arg("logits"), py::arg("targets"), py::arg("ignore"),
+        py::arg("reduction"), py::arg("scaled"), py::arg("twice") = false);
   m.def("token_log_probs", &mgx::token_log_probs,
         "Log probabilities of given tokens, entropy, best alternatives");
 }

@@ -14,7 +14,7 @@ other target outside the classes is an IndexError on the CPU; on a GPU,
 where finding it would take a synchronisation, nothing is read for it and
 its value and its row of the gradient are NaN. A logit of -inf is a masked
 class: probability 0, gradient 0. A row with a NaN, a +inf or nothing but
--inf gives NaN. Neither function has a second derivative.
+-inf gives NaN. Neither function has a second derivative; the module has.
 """
 from __future__ import annotations
 
@@ -24,7 +24,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .grad_clip import load_lm
+from .grad_clip import load_lm, seen_whole
 
 TokenLogProbs = collections.namedtuple(
     'TokenLogProbs', ['log_probs', 'entropy', 'top_log_probs', 'top_ids'])
@@ -92,20 +92,24 @@ def _check(logits, targets):
 
 class MgxCrossEntropyLoss(nn.CrossEntropyLoss):
     """nn.CrossEntropyLoss on the HIP kernels for (N, classes) logits and
-    class indices; the loss is float32 whatever the logits' type. Weights,
-    label smoothing, class probabilities and other shapes go to torch."""
+    class indices, with second and further derivatives; the loss is float32
+    whatever the logits' type. Weights, label smoothing, class
+    probabilities, other shapes, and calls that torch has to see as its own
+    operations (torch.compile and tracing, torch.func, forward-mode
+    differentiation) go to torch."""
 
     def _use_hip_path(self, x, y):
         return (x.is_cuda and x.dtype in _TYPES and x.dim() == 2
                 and y.dim() == 1 and y.dtype in (torch.int64, torch.int32)
                 and x.size(0) == y.size(0) and self.weight is None
-                and self.label_smoothing == 0.0)
+                and self.label_smoothing == 0.0 and seen_whole(x, y))
 
     def forward(self, x, y):
         if not self._use_hip_path(x, y):
             return super().forward(x, y)
-        return cross_entropy(x, y, ignore_index=self.ignore_index,
-                             reduction=self.reduction)
+        return load_lm().cross_entropy(x, y, self.ignore_index,
+                                       _REDUCTIONS[self.reduction], False,
+                                       True)
 
 
 # --------------------------------------------------------------------------

@@ -46,8 +46,10 @@
 #include "lm_common.h"
 
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
+#include <limits>
 #include <tuple>
 #include <vector>
 
@@ -1016,6 +1018,8 @@ torch::Tensor as_rows(const torch::Tensor& logits) {
 }
 
 void check_inputs(const torch::Tensor& logits, const torch::Tensor& targets) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(),
+              "the token loss kernels cannot be traced");
   TORCH_CHECK_VALUE(logits.is_cuda(), "logits must be on a GPU");
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 &&
                         logits.size(-1) < (1L << 30),
@@ -1242,14 +1246,83 @@ void refuse_second_order() {
               "differentiated with create_graph=True");
 }
 
+GradIn loss_grad_in(const torch::Tensor& g, const torch::Tensor& targets,
+                    const torch::Tensor& work, long rows, long ignore,
+                    bool none) {
+  const float* w = work.data_ptr<float>();
+  return GradIn{reinterpret_cast<const float2*>(w), nullptr,
+                targets.data_ptr(), is_wide(targets), ignore,
+                g.data_ptr<float>(), none ? (long)g.stride(0) : 0L,
+                none ? nullptr : w + 3 * rows, -1.f, nullptr, 0L};
+}
+
+// The loss's gradient as a function of the logits and of the gradient g
+// that comes in, d_j = c (p_j - [j = t]) with c = g, times a mean's share.
+// For a gradient e of d that comes in in turn, with m = sum_j p_j e_j:
+//
+//   of x_j: c p_j (e_j - m)        of g: share (m - e_t), summed over the
+//                                  rows where g is one for all
+//
+// This is rare, and made of torch's own operations, which can be
+// differentiated further.
+struct CrossEntropyGrad : torch::autograd::Function<CrossEntropyGrad> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x,
+                               torch::Tensor grad, torch::Tensor targets,
+                               torch::Tensor work, int64_t ignore,
+                               bool none) {
+    c10::DeviceGuard guard(x.device());
+    ctx->save_for_backward({x, grad, targets, work});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["none"] = none;
+    const auto g = flat_grad(grad);
+    return grad_of(x, loss_grad_in(g, targets, work, x.size(0), ignore,
+                                   none));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto& x = saved[0];
+    const auto& targets = saved[2];
+    const bool none = ctx->saved_data["none"].toBool();
+    c10::DeviceGuard guard(x.device());
+    const auto kept = targets.ne(ctx->saved_data["ignore"].toInt());
+    const auto there = targets.ge(0).logical_and(targets.lt(x.size(1)));
+    // a row that takes no part may be anything; it is left out first
+    const auto p = x.to(at::kFloat)
+                       .masked_fill(kept.logical_not().unsqueeze(1), 0)
+                       .softmax(1);
+    const auto e = grads[0].to(at::kFloat);
+    const auto m = (p * e).sum(1, true);
+    auto c = kept.logical_and(there).to(at::kFloat);
+    c = c.masked_fill(kept.logical_and(there.logical_not()),
+                      std::numeric_limits<float>::quiet_NaN());
+    if (!none) c = c * saved[3][3 * x.size(0)];
+    const auto g = saved[1].to(at::kFloat);
+    const auto at = targets.to(at::kLong)
+                        .masked_fill(there.logical_not(), 0).unsqueeze(1);
+    auto dg = (c.unsqueeze(1) * (m - e.gather(1, at))).squeeze(1)
+                  .masked_fill(kept.logical_not(), 0);
+    if (!none) dg = dg.sum();
+    const auto dx = ((c * g).unsqueeze(1) * p * (e - m))
+                        .masked_fill(kept.logical_not().unsqueeze(1), 0);
+    return {dx.to(x.scalar_type()), dg.to(saved[1].scalar_type()),
+            torch::Tensor(), torch::Tensor(), torch::Tensor(),
+            torch::Tensor()};
+  }
+};
+
 // The forward pass leaves the gradient for an incoming 1, and the first
 // backward pass hands it on. A second one works it out again, since by then
 // it is the caller's own; so does one that is captured into another graph
 // than the forward pass, which may be replayed alone.
+//
+// `twice`: the backward pass may itself be differentiated; it is then a
+// function of its own.
 struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x,
                                torch::Tensor targets, int64_t ignore,
-                               int64_t reduction, bool with_grad) {
+                               int64_t reduction, bool with_grad,
+                               bool twice) {
     c10::DeviceGuard guard(x.device());
     const long rows = x.size(0);
     const auto f32 = x.options().dtype(torch::kFloat);
@@ -1281,6 +1354,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     ctx->save_for_backward({x, targets, work});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["twice"] = twice;
     if (ready.defined()) {
       ctx->saved_data["capture"] = (int64_t)capture_id();
       ctx->saved_data["ready"] = ready;
@@ -1289,19 +1363,21 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    refuse_second_order();
     const auto saved = ctx->get_saved_variables();
     const auto& x = saved[0];
-    c10::DeviceGuard guard(x.device());
-    const long rows = x.size(0);
-    const auto g = flat_grad(grads[0]);
-    const float* work = saved[2].data_ptr<float>();
     const bool none = ctx->saved_data["reduction"].toInt() == kNone;
-    GradIn in{reinterpret_cast<const float2*>(work), nullptr,
-              saved[1].data_ptr(), is_wide(saved[1]),
-              (long)ctx->saved_data["ignore"].toInt(), g.data_ptr<float>(),
-              none ? (long)g.stride(0) : 0L, none ? nullptr : work + 3 * rows,
-              -1.f, nullptr, 0L};
+    const int64_t ignore = ctx->saved_data["ignore"].toInt();
+    if (at::GradMode::is_enabled()) {
+      if (!ctx->saved_data["twice"].toBool()) refuse_second_order();
+      return {CrossEntropyGrad::apply(x, grads[0], saved[1], saved[2], ignore,
+                                      none),
+              torch::Tensor(), torch::Tensor(), torch::Tensor(),
+              torch::Tensor(), torch::Tensor()};
+    }
+    c10::DeviceGuard guard(x.device());
+    const auto g = flat_grad(grads[0]);
+    const GradIn in = loss_grad_in(g, saved[1], saved[2], x.size(0), ignore,
+                                   none);
     torch::Tensor ready;
     const auto at = ctx->saved_data.find("ready");
     if (at != ctx->saved_data.end() &&
@@ -1310,7 +1386,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
       ctx->saved_data.erase("ready");
     }
     return {grad_of(x, in, ready), torch::Tensor(), torch::Tensor(),
-            torch::Tensor(), torch::Tensor()};
+            torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
 };
 
@@ -1361,7 +1437,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
 
 torch::Tensor cross_entropy(const torch::Tensor& logits,
                             const torch::Tensor& targets, int64_t ignore,
-                            int64_t reduction, bool scaled) {
+                            int64_t reduction, bool scaled, bool twice) {
   check_inputs(logits, targets);
   TORCH_CHECK_VALUE(reduction >= kNone && reduction <= kSum,
                     "unknown reduction ", reduction);
@@ -1369,7 +1445,7 @@ torch::Tensor cross_entropy(const torch::Tensor& logits,
   c10::DeviceGuard guard(logits.device());
   auto loss = CrossEntropy::apply(
       as_rows(logits), targets.reshape({-1}).contiguous(), ignore, reduction,
-      !scaled && at::GradMode::is_enabled() && logits.requires_grad());
+      !scaled && at::GradMode::is_enabled() && logits.requires_grad(), twice);
   return reduction == kNone && targets.dim() != 1
       ? loss.view(targets.sizes()) : loss;
 }

@@ -368,3 +368,75 @@ def test_together_the_trainer():
                 out.view(-1, 10000), y.cuda().view(-1)).item()
     assert abs(math.log(ppl) - total / 2) < 1e-4
     assert 0.0 <= t.top5_accuracy <= 1.0 and t.mean_entropy > 0.0
+
+
+# The module is in a model, in the place of nn.Embedding: what could be done
+# with that model has to go on. Products and sums of a few terms in float32,
+# on either side: U for each.
+
+def _pair(**kw):
+    """An MgxEmbedding and torch's with the same weights, and tokens."""
+    torch.manual_seed(6)
+    a = em.MgxEmbedding(13, 5, **kw).cuda()
+    b = torch.nn.Embedding(13, 5, **kw).cuda()
+    b.load_state_dict(a.state_dict())
+    return a, b, _tokens(40, 13, 'text').view(4, 10)
+
+
+@pytest.mark.parametrize('pad', [None, 1])
+@pytest.mark.parametrize('scale', [1.0, 2.0])
+def test_module_has_higher_derivatives(pad, scale):
+    a, b, t = _pair(padding_idx=pad)
+    a.scale = scale
+    c = torch.randn(4, 10, 5, device='cuda')
+    v = torch.randn(13, 5, device='cuda')
+    out = []
+    for m, k in ((a, 1.0), (b, scale)):
+        y = ((m(t) * k) ** 3 * c).sum()
+        g, = torch.autograd.grad(y, m.weight, create_graph=True)
+        h, = torch.autograd.grad((g * v).sum(), m.weight, create_graph=True)
+        i, = torch.autograd.grad((h * v).sum(), m.weight)
+        out.append((g.detach(), h.detach(), i))
+    for x, y in zip(*out):
+        assert torch.allclose(x, y, rtol=1e-5, atol=1e-4)
+        if pad is not None:
+            assert bool((x[pad] == 0).all())
+
+
+def test_module_under_transforms():
+    """torch.func, forward-mode differentiation, tracing, compiling and
+    tensors without data see torch's own embedding."""
+    a, b, t = _pair()
+    w = a.weight.detach()
+
+    def total(m):
+        return lambda w: (torch.func.functional_call(
+            m, {'weight': w}, (t,)) ** 2).sum()
+
+    assert torch.allclose(torch.func.grad(total(a))(w),
+                          torch.func.grad(total(b))(w), rtol=1e-5)
+    ws = torch.randn(3, 13, 5, device='cuda')
+    assert torch.allclose(torch.func.vmap(total(a))(ws),
+                          torch.func.vmap(total(b))(ws), rtol=1e-5)
+    v = torch.randn(13, 5, device='cuda')
+    for x, y in zip(torch.func.jvp(total(a), (w,), (v,)),
+                    torch.func.jvp(total(b), (w,), (v,))):
+        assert torch.allclose(x, y, rtol=1e-5)
+    traced = torch.jit.trace(a, (t,))
+    u = (t + 1) % 13
+    assert torch.equal(traced(u), b(u))
+    compiled = torch.compile(a, fullgraph=True, backend='eager')
+    assert torch.equal(compiled(u), b(u))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        y = a(mode.from_tensor(t))
+    assert y.shape == (4, 10, 5)
+    assert torch.equal(a(t), b(t))
+
+
+def test_function_refuses_to_be_traced():
+    """A trace would not see the kernel, and its outputs would not be
+    computed."""
+    w, t = _weight(9, 4, F32), torch.tensor([1, 2], device='cuda')
+    with pytest.raises(RuntimeError):
+        torch.jit.trace(lambda t: em.embedding(t, w), (t,))

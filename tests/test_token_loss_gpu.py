@@ -644,3 +644,83 @@ def test_statistics_of_peaked_rows(vocab, kind):
             {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126,
              torch.float16: 2.0 ** -24}[kind]
         assert bool(((got.double() - want).abs() <= off).all()), i
+
+
+# The module stands where nn.CrossEntropyLoss stood: what could be done with
+# it has to go on. REL covers the sums of float32 on either side.
+
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('vocab', [7, 2500])
+def test_module_has_higher_derivatives(vocab, reduction):
+    x, t = _make(6, vocab, torch.float32, seed=40, scale=1.0)
+    t[2] = -100
+    w = torch.rand(6, device='cuda') + 0.5
+    v = torch.randn(6, vocab, device='cuda')
+    out = []
+    for loss, kind in ((tl.MgxCrossEntropyLoss(reduction=reduction), x.dtype),
+                       (torch.nn.CrossEntropyLoss(reduction=reduction),
+                        torch.float64)):
+        y = x.to(kind).requires_grad_(True)
+        k = w.to(kind).requires_grad_(True)
+        l = loss(y, t)
+        l = (l * (k if reduction == 'none' else k.sum())).sum()
+        g, = torch.autograd.grad(l, y, create_graph=True)
+        hx, hk = torch.autograd.grad((g * v).sum(), (y, k),
+                                     create_graph=True)
+        i, = torch.autograd.grad((hx * v).sum(), y)
+        out.append([z.detach().double() for z in (g, hx, hk, i)])
+    for a, b in zip(*out):
+        assert torch.allclose(a, b, rtol=4 * REL,
+                              atol=4 * REL * float(b.abs().max()))
+    assert bool((out[0][0][2] == 0).all()) and bool((out[0][1][2] == 0).all())
+
+
+def test_module_first_derivative_with_a_graph():
+    """create_graph=True changes nothing in the gradient itself, masked
+    classes and ignored rows that are not finite among it."""
+    x, t = _make(5, 1003, torch.bfloat16, seed=41)
+    x[0, 5:] = NEG
+    t[0] = 2
+    x[3] = float('nan')
+    t[3] = -100
+    x.requires_grad_(True)
+    loss = tl.MgxCrossEntropyLoss()(x, t)
+    a, = torch.autograd.grad(loss, x, create_graph=True)
+    b, = torch.autograd.grad(tl.MgxCrossEntropyLoss()(x, t), x)
+    assert torch.allclose(a.detach().float(), b.float(),
+                          rtol=torch.finfo(torch.bfloat16).eps, atol=0)
+    v = torch.randn(5, 1003, device='cuda').bfloat16()
+    h, = torch.autograd.grad((a * v).sum(), x)
+    assert torch.isfinite(h).all()
+    assert bool((h[3] == 0).all()) and bool((h[0, 5:] == 0).all())
+
+
+def test_module_under_transforms():
+    x, t = _make(12, 50, torch.float32, seed=42)
+    a, b = tl.MgxCrossEntropyLoss(), torch.nn.CrossEntropyLoss()
+    v = torch.randn_like(x)
+    close = dict(rtol=1e-5, atol=1e-6)
+    assert torch.allclose(torch.func.grad(lambda y: a(y, t))(x),
+                          torch.func.grad(lambda y: b(y, t))(x), **close)
+    assert torch.allclose(
+        torch.func.vmap(a)(x.view(3, 4, 50), t.view(3, 4)),
+        torch.func.vmap(b)(x.view(3, 4, 50), t.view(3, 4)), **close)
+    for p, q in zip(torch.func.jvp(lambda y: a(y, t), (x,), (v,)),
+                    torch.func.jvp(lambda y: b(y, t), (x,), (v,))):
+        assert torch.allclose(p, q, **close)
+    y, u = _make(12, 50, torch.float32, seed=43)
+    traced = torch.jit.trace(a, (x, t))
+    assert torch.allclose(traced(y, u), b(y, u), **close)
+    compiled = torch.compile(a, fullgraph=True, backend='eager')
+    assert torch.allclose(compiled(y, u), b(y, u), **close)
+    assert torch.allclose(a(y, u), b(y, u), **close)
+
+
+def test_functions_refuse_to_be_traced():
+    """A trace would not see the kernels, and its outputs would not be
+    computed."""
+    x, t = _make(3, 20, torch.float32)
+    for call in (lambda x, t: tl.cross_entropy(x, t),
+                 lambda x, t: tl.token_log_probs(x, t).log_probs):
+        with pytest.raises(RuntimeError):
+            torch.jit.trace(call, (x, t))
