@@ -136,8 +136,40 @@ def token_log_probs_reference(logits, targets, top_k=0, ignore_index=-100):
         raise IndexError('a target is outside the classes')
     lp = torch.where(keep, log.gather(-1, at.unsqueeze(-1)).squeeze(-1),
                      torch.zeros((), dtype=log.dtype, device=log.device))
-    finite = log.masked_fill(log == float('-inf'), 0.0)
-    entropy = -(log.exp() * finite).sum(-1)
-    ids = torch.sort(logits.detach(), dim=-1, descending=True,
-                     stable=True)[1][..., :top_k]
-    return TokenLogProbs(lp, entropy, log.detach().gather(-1, ids), ids)
+    ids = _best(logits.detach(), top_k)
+    top = log.detach().gather(-1, ids)
+    # a class of probability 0 adds nothing: 0 times the lowest value
+    low = torch.finfo(log.dtype).min
+    if log.requires_grad:
+        entropy = -(log.exp() * log.clamp(min=low)).sum(-1)
+    else:
+        # in place: 700 x 10000 take 4 ms, and 11 with new memory each time
+        entropy = -log.exp().mul_(log.clamp_(min=low)).sum(-1)
+    return TokenLogProbs(lp, entropy, top, ids)
+
+
+def _best(x, k):
+    """Indices of the ``k`` largest values of each row, best first, of equal
+    ones the lowest index first; a NaN is larger than any other. torch.topk
+    finds them where no two of the best ``k + 1`` are equal. In the other
+    rows as many of those equal to the last are taken as there is room for,
+    from the left, and only what is left is sorted: 700 rows of 10000 and
+    their best five take 5 ms on eight cores, where sorting them whole takes
+    130."""
+    v, ids = torch.topk(x, min(k + 1, x.size(-1)))
+    ids = ids[..., :k].contiguous()
+    same = ((v[..., 1:] == v[..., :-1]) | v[..., 1:].isnan()).any(-1)
+    if k == 0 or not bool(same.any()):
+        return ids
+    y = x[same]
+    last = v[same][:, k - 1:k]
+    nan, no_last = y.isnan(), last.isnan()
+    above = (y > last) | (nan & ~no_last)
+    equal = (y == last) | (nan & no_last)
+    room = k - above.sum(-1, keepdim=True)
+    keep = above | (equal & (equal.cumsum(-1) <= room))
+    at = keep.nonzero()[:, 1].view(-1, k)
+    order = torch.sort(y.gather(1, at), dim=-1, descending=True,
+                       stable=True)[1]
+    ids[same] = at.gather(1, order)
+    return ids

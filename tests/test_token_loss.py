@@ -120,3 +120,51 @@ def test_word_level_evaluation():
     assert 0.0 <= t.top5_accuracy <= 1.0
     # nearly uniform over 10000 words
     assert t.mean_entropy == pytest.approx(math.log(10000), rel=0.05)
+
+
+def _rows_with_ties(kind):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(9, 200, generator=g).to(kind)
+    x[1] = x[1].round()                  # many equal values
+    x[2] = 0.0
+    x[3, ::2] = -0.0
+    x[3, 1::2] = 0.0                     # both zeros are the same value
+    x[4, 7] = float('nan')
+    x[5, 3:90] = float('nan')
+    x[6, 4:] = NEG
+    x[7, 11] = x[7, 150] = float('inf')
+    x[8, 100] = x[8].max()               # the best one twice
+    return x.view(3, 3, 200)
+
+
+@pytest.mark.parametrize('kind', [torch.float32, torch.float64,
+                                  torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('k', [0, 1, 2, 5, 64])
+def test_best_of_equal_values(kind, k):
+    x = _rows_with_ties(kind)
+    r = tl.token_log_probs_reference(
+        x, torch.zeros(3, 3, dtype=torch.long), top_k=k)
+    ids = torch.sort(x, dim=-1, descending=True, stable=True)[1][..., :k]
+    assert torch.equal(r.top_ids, ids)
+    all_of_them = tl.token_log_probs_reference(
+        x[..., :64], torch.zeros(3, 3, dtype=torch.long), top_k=64)
+    assert torch.equal(all_of_them.top_ids, torch.sort(
+        x[..., :64], dim=-1, descending=True, stable=True)[1])
+
+
+def test_best_without_sorting_the_row():
+    """A few of many classes: the rows are never sorted whole."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    longest = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, f, types, args=(), kwargs=None):
+            if 'sort' in str(f):
+                longest.append(args[0].size(-1))
+            return f(*args, **(kwargs or {}))
+
+    with Log():
+        for kind in (torch.float32, torch.bfloat16):
+            tl.token_log_probs(_rows_with_ties(kind),
+                               torch.zeros(3, 3, dtype=torch.long), top_k=5)
+    assert max(longest, default=0) <= 5
