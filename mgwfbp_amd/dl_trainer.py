@@ -585,11 +585,13 @@ class DLTrainer:
                     score = (token_log_probs if settings.USE_HIP_KERNELS
                              else token_log_probs_reference)
                     r = score(out, y, top_k=min(5, self.net.ntokens))
-                    # accumulated on the device, read back at the end
-                    total_loss -= r.log_probs.mean()
-                    total_entropy += r.entropy.mean()
+                    # accumulated on the device, in 64 bits, and read back
+                    # at the end
+                    f64 = torch.float64
+                    total_loss -= r.log_probs.mean(dtype=f64)
+                    total_entropy += r.entropy.mean(dtype=f64)
                     total_top5 += (r.top_ids == y.unsqueeze(-1)).any(
-                        -1).float().mean()
+                        -1).to(f64).mean()
                     nbatches += 1
                     continue
                 x, y = batch

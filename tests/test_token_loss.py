@@ -168,3 +168,48 @@ def test_best_without_sorting_the_row():
             tl.token_log_probs(_rows_with_ties(kind),
                                torch.zeros(3, 3, dtype=torch.long), top_k=5)
     assert max(longest, default=0) <= 5
+
+
+def _word_level(batches, ntokens=40):
+    """A DLTrainer whose word-level model gives the logits of ``batches``,
+    (logits, targets) of 4 sequences each, in turn."""
+    from mgwfbp_amd.dl_trainer import DLTrainer
+    t = DLTrainer(rank=0, size=1, dist=False, batch_size=4, ngpus=0,
+                  data_dir='', dataset='ptb', dnn='lstm', lr=1.0, nworkers=1,
+                  prefix='t', synthetic=True)
+
+    class Net(torch.nn.Module):
+        batch_size = 4
+
+        def __init__(self):
+            super().__init__()
+            self.ntokens = ntokens
+            self.given = iter([x for x, _ in batches])
+
+        def init_hidden(self):
+            return None
+
+        def forward(self, x, hidden):
+            return next(self.given), hidden
+
+    t.net = Net()
+    t.testloader = [(y, y) for _, y in batches]
+    return t
+
+
+def test_evaluation_sums_in_64_bits():
+    """Many batches with losses near 10: a float32 sum past 2^14 loses 2^-10
+    of each, and the perplexity's exponent with it. Each batch's mean is a
+    float32, off by half a step of the loss for each of a few roundings."""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 3, 40, generator=g) * 4.0
+    y = torch.randint(0, 40, (4, 3), generator=g)
+    x.scatter_(-1, y.unsqueeze(-1), -12.0)
+    n = 4000
+    t = _word_level([(x, y)] * n)
+    ppl = t.test(0)
+    log = torch.log_softmax(x.double(), -1)
+    want = -float(log.gather(-1, y.unsqueeze(-1)).mean())
+    h = -float((log.exp() * log).sum(-1).mean())
+    assert abs(math.log(ppl) - want) <= 8 * 2.0 ** -24 * want
+    assert abs(t.mean_entropy - h) <= 64 * 2.0 ** -24 * h
