@@ -584,14 +584,19 @@ class DLTrainer:
                     out, _ = self.net(x, hidden)
                     score = (token_log_probs if settings.USE_HIP_KERNELS
                              else token_log_probs_reference)
-                    r = score(out, y, top_k=min(5, self.net.ntokens))
+                    r = score(out, y, top_k=min(5, self.net.ntokens),
+                              ignore_index=self.criterion.ignore_index)
+                    # means over the targets that are not ignored,
                     # accumulated on the device, in 64 bits, and read back
                     # at the end
                     f64 = torch.float64
-                    total_loss -= r.log_probs.mean(dtype=f64)
-                    total_entropy += r.entropy.mean(dtype=f64)
-                    total_top5 += (r.top_ids == y.unsqueeze(-1)).any(
-                        -1).to(f64).mean()
+                    kept = y != self.criterion.ignore_index
+                    n = kept.sum(dtype=f64)
+                    total_loss -= r.log_probs.sum(dtype=f64) / n
+                    total_entropy += r.entropy.masked_fill(
+                        ~kept, 0.0).sum(dtype=f64) / n
+                    hits = (r.top_ids == y.unsqueeze(-1)).any(-1)
+                    total_top5 += hits.sum(dtype=f64) / n
                     nbatches += 1
                     continue
                 x, y = batch

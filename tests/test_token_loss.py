@@ -213,3 +213,25 @@ def test_evaluation_sums_in_64_bits():
     h = -float((log.exp() * log).sum(-1).mean())
     assert abs(math.log(ppl) - want) <= 8 * 2.0 ** -24 * want
     assert abs(t.mean_entropy - h) <= 64 * 2.0 ** -24 * h
+
+
+def test_evaluation_leaves_ignored_targets_out():
+    """As the mean cross entropy does: neither in the loss nor in what it is
+    divided by, nor among the five best."""
+    g = torch.Generator().manual_seed(2)
+    batches = []
+    want = []
+    hits = []
+    for i in range(3):
+        x = torch.randn(4, 5, 40, generator=g)
+        y = torch.randint(0, 40, (4, 5), generator=g)
+        y[:, 4 - i:] = -100
+        batches.append((x, y))
+        want.append(float(torch.nn.functional.cross_entropy(
+            x.double().view(-1, 40), y.view(-1))))
+        kept = y != -100
+        hits.append(float((x.topk(5)[1] == y.unsqueeze(-1)).any(-1)[kept]
+                          .double().mean()))
+    t = _word_level(batches)
+    assert math.log(t.test(0)) == pytest.approx(sum(want) / 3, rel=1e-6)
+    assert t.top5_accuracy == pytest.approx(sum(hits) / 3, abs=1e-12)
