@@ -552,11 +552,12 @@ void multi_tensor_sgd(torch::Tensor t_tensors, torch::Tensor t_chunks,
 }
 
 // The update with the gradients clipped by their global norm; returns the
-// norm, float32, on the device.
+// norm, float32, on the device. `past`: the parameters are too many for the
+// gradients to stay in the 256 MB cache between the two passes.
 torch::Tensor multi_tensor_sgd_clipped(
     torch::Tensor t_tensors, torch::Tensor t_chunks, long nchunks, double lr,
     torch::Tensor lr_buf, double momentum, double dampening, bool nesterov,
-    double grad_scale, double max_norm, double eps) {
+    double grad_scale, double max_norm, double eps, bool past) {
   c10::DeviceGuard guard(t_tensors.device());
   auto stream = c10::hip::getCurrentHIPStream().stream();
   const float* lr_ptr =
@@ -569,9 +570,6 @@ torch::Tensor multi_tensor_sgd_clipped(
   const int nparts = std::max(1, std::min((int)nchunks, 1024));
   auto partials = torch::empty({nparts}, opts.dtype(torch::kDouble));
   auto norm = torch::empty({}, opts.dtype(torch::kFloat));
-  // what the chunks can hold at most; the update past the cache from 128 MB
-  // of parameters on
-  const bool past = nchunks * kChunk * (long)sizeof(float) >= (128L << 20);
   const auto sums = past ? sgd_norm_partials_kernel<true>
                          : sgd_norm_partials_kernel<false>;
   const auto update = past ? multi_tensor_sgd_kernel<true, true>

@@ -307,3 +307,24 @@ class TestClippedStep:
         ob.step()
         for p, q in zip(a.parameters(), b.parameters()):
             assert torch.allclose(p, q, rtol=1e-6, atol=1e-7)
+
+
+def test_step_of_many_small_tensors_uses_the_cache():
+    """What goes past the cache is decided by the parameters' size, not by
+    their number."""
+    n = 700
+    shapes = [(i % 37 + 1,) for i in range(n)]
+    params = _grads(shapes, [F32] * n, seed=1)
+    grads = _grads(shapes, [F32] * n, seed=2)
+    want = [p.double() for p in params]
+    norm = sum(float(g.double().square().sum()) for g in grads) ** 0.5
+    sgd = K.FusedSGD(params, grads, [], [0.0] * n)
+    assert not sgd._past
+    got = sgd.step(0.5, max_norm=0.25)
+    assert abs(float(got) - norm) <= 1.01 * HALF * norm
+    f = min(1.0, 0.25 / (norm + 1e-6))
+    for p, w, g in zip(params, want, grads):
+        step = 0.5 * f * g.double()
+        most = w.abs() + step.abs()
+        assert bool(((p.double() - (w - step)).abs()
+                     <= 8 * HALF * most).all())
