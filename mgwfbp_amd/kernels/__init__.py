@@ -100,13 +100,13 @@ class FusedSGD:
                  momentum=0.0, dampening=0.0, nesterov=False):
         self.ext = load_kernels(required=True)
         assert self.ext is not None
-        params = list(params)
+        params, grads, momenta = list(params), list(grads), list(momenta)
+        self._tensors = params, grads, momenta  # the table has addresses only
         self.momentum = momentum
         self.dampening = dampening
         self.nesterov = nesterov
         t_tensors, t_chunks, t_n = self.ext.build_sgd_table(
-            params, list(grads),
-            list(momenta) if momentum != 0.0 else [],
+            params, grads, momenta if momentum != 0.0 else [],
             [float(w) for w in weight_decays])
         self._t_tensors = t_tensors
         self._t_chunks = t_chunks
@@ -158,8 +158,9 @@ class PackTable:
     def __init__(self, tensors, offsets):
         self.ext = load_kernels(required=True)
         assert self.ext is not None
+        self._tensors = list(tensors)           # the table has addresses only
         t_descs, t_chunks, t_n = self.ext.build_pack_table(
-            list(tensors), [int(o) for o in offsets])
+            self._tensors, [int(o) for o in offsets])
         self._t_descs = t_descs
         self._t_chunks = t_chunks
         self._nchunks = int(t_n.item())

@@ -106,3 +106,34 @@ def test_single_process_entry_uses_the_clipped_step():
     from mgwfbp_amd import dist_trainer
     assert 'max_grad_norm' in inspect.getsource(dist_trainer.mgwfbp)
     assert K.FusedSGD.step.__doc__
+
+
+class _NoKernels:
+    """Stands for the extension where tables are built: on the host."""
+
+    def build_sgd_table(self, *args):
+        return torch.zeros(1), torch.zeros(1), torch.ones(1)
+
+    build_pack_table = build_sgd_table
+
+
+def test_tables_keep_their_tensors(monkeypatch):
+    """A table holds addresses, which have to stay the tensors' own for as
+    long as it is used, whatever the caller lets go of."""
+    import gc
+    import weakref
+    monkeypatch.setattr(K, 'load_kernels', lambda required=None: _NoKernels())
+
+    def new():
+        return [torch.zeros(3), torch.zeros(2)]
+
+    p, g, m, s = new(), new(), new(), new()
+    alive = [weakref.ref(t) for t in p + g + m + s]
+    tables = (K.FusedSGD(p, g, m, [0.0, 0.0], momentum=0.9),
+              K.PackTable(s, [0, 64]))
+    del p, g, m, s
+    gc.collect()
+    assert all(r() is not None for r in alive)
+    del tables
+    gc.collect()
+    assert all(r() is None for r in alive)
