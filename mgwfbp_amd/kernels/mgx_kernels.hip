@@ -498,13 +498,31 @@ std::vector<torch::Tensor> build_sgd_table(
     const std::vector<double>& wds) {
   const int nt = params.size();
   TORCH_CHECK(nt > 0, "empty tensor list");
+  // the kernels go by the addresses and by the parameters' sizes
+  TORCH_CHECK((int)grads.size() == nt && (int)wds.size() == nt &&
+                  (momenta.empty() || (int)momenta.size() == nt),
+              "fused SGD needs a gradient, a weight decay and, with "
+              "momentum, a buffer for each parameter");
+  const auto fits = [&](const torch::Tensor& t, const torch::Tensor& p) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat,
+                "fused SGD expects fp32 master params, gradients and "
+                "momentum buffers");
+    TORCH_CHECK(t.is_contiguous(), "fused SGD expects contiguous tensors");
+    TORCH_CHECK(t.numel() == p.numel(),
+                "fused SGD expects a parameter's gradient and momentum "
+                "buffer to be of its size");
+    TORCH_CHECK(t.is_cuda() && t.device() == params[0].device(),
+                "fused SGD expects all tensors on one GPU");
+  };
+  for (int i = 0; i < nt; ++i) {
+    fits(params[i], params[i]);
+    fits(grads[i], params[i]);
+    if (!momenta.empty()) fits(momenta[i], params[i]);
+  }
+  c10::DeviceGuard guard(params[0].device());
   std::vector<TensorTriple> triples(nt);
   std::vector<Chunk> chunks;
   for (int i = 0; i < nt; ++i) {
-    TORCH_CHECK(params[i].is_contiguous() && grads[i].is_contiguous(),
-                "params/grads must be contiguous");
-    TORCH_CHECK(params[i].scalar_type() == at::kFloat,
-                "fused SGD expects fp32 master params");
     triples[i].p = params[i].data_ptr<float>();
     triples[i].g = grads[i].data_ptr<float>();
     triples[i].m =

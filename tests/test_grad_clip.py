@@ -137,3 +137,25 @@ def test_tables_keep_their_tensors(monkeypatch):
     del tables
     gc.collect()
     assert all(r() is None for r in alive)
+
+
+@pytest.mark.parametrize('p,g,m,wd', [
+    ([3, 2], [3], [], 2), ([3], [2], [], 1), ([3], [3], [2], 1),
+    ([3, 2], [3, 2], [3], 2), ([3], [3], [], 0), ([3], [3], [], 1)])
+def test_update_table_refuses_lists_that_do_not_fit(p, g, m, wd):
+    """The kernels go by the parameters' sizes; the last list fits, but lies
+    on the host."""
+    def new(sizes):
+        return [torch.zeros(n) for n in sizes]
+    with pytest.raises((ValueError, RuntimeError), match='fused SGD'):
+        K.FusedSGD(new(p), new(g), new(m), [0.0] * wd, momentum=0.5 if m
+                   else 0.0)
+
+
+def test_update_table_refuses_other_types():
+    half = [torch.zeros(3, dtype=torch.bfloat16)]
+    full = [torch.zeros(3)]
+    for p, g, m in ((half, full, full), (full, half, full),
+                    (full, full, half)):
+        with pytest.raises((ValueError, RuntimeError), match='fused SGD'):
+            K.FusedSGD(p, g, m, [0.0], momentum=0.5)
