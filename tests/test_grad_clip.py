@@ -159,3 +159,57 @@ def test_update_table_refuses_other_types():
                     (full, full, half)):
         with pytest.raises((ValueError, RuntimeError), match='fused SGD'):
             K.FusedSGD(p, g, m, [0.0], momentum=0.5)
+
+
+@pytest.mark.parametrize('dnn,dataset,limit', [('lstm', 'ptb', 0.25),
+                                               ('lstman4', 'an4', 400)])
+def test_single_process_entry_clips(monkeypatch, dnn, dataset, limit):
+    """The entry as it runs, with smaller networks: each update is given the
+    model's limit, and the word-level model's is plain SGD with the
+    gradients scaled to it. A parameter's update has four roundings, of the
+    rate, two products and the difference: of the parameter's size for the
+    last, and of the step's for the others; a product below the smallest
+    normal number is off by half of 2^-149 instead, and a word of next to no
+    probability has such a gradient, for a bias that is 0."""
+    from mgwfbp_amd import dist_trainer, dl_trainer, models, settings
+    monkeypatch.setattr(settings, 'ADAPTIVE_MERGE', False)
+    torch.manual_seed(0)
+    create = dl_trainer.create_net
+
+    def small(num_classes, name, **kw):
+        if name == 'lstm':
+            net = models.lstm(vocab_size=kw['vocab_size'], embedding_dim=6,
+                              hidden_dim=6, batch_size=kw['batch_size'])
+            with torch.no_grad():        # gradients well above the limit
+                net.fc.weight.mul_(300.0)
+                net.rnn.bias_ih_l1.fill_(2.0)
+            return net, None
+        return create(num_classes, name, **kw)
+
+    monkeypatch.setattr(dl_trainer, 'create_net', small)
+    seen = []
+
+    class Trainer(dl_trainer.DLTrainer):
+        def update_model(self, max_grad_norm=None):
+            params = [p for p in self.net.parameters()]
+            before = [p.detach().clone() for p in params]
+            grads = [p.grad.double() for p in params]
+            norm = sum(float(g.square().sum()) for g in grads) ** 0.5
+            super().update_model(max_grad_norm=max_grad_norm)
+            seen.append((max_grad_norm, norm))
+            if dnn != 'lstm':
+                return
+            f = min(1.0, max_grad_norm / (norm + 1e-6))
+            for p, b, g in zip(params, before, grads):
+                step = self.lr * f * g
+                off = (p.detach().double() - (b.double() - step)).abs()
+                most = 4 * 2.0 ** -24 * (b.double().abs() + step.abs()) \
+                    + 2.0 ** -149
+                assert bool((off <= most).all())
+
+    monkeypatch.setattr(dist_trainer, 'DLTrainer', Trainer)
+    dist_trainer.mgwfbp(dnn, dataset, '', 1, 0.5, 2, 1, max_epochs=1,
+                        num_steps=5, max_iters=2)
+    assert [m for m, _ in seen] == [limit, limit]
+    if dnn == 'lstm':
+        assert all(n > limit for _, n in seen)
