@@ -328,3 +328,67 @@ def test_step_of_many_small_tensors_uses_the_cache():
         most = w.abs() + step.abs()
         assert bool(((p.double() - (w - step)).abs()
                      <= 8 * HALF * most).all())
+
+
+class TestPastTheCache:
+    """From 128 MB on the gradients go past the cache, by other variants of
+    the kernels, compared here on the GPU in 64 bits."""
+
+    SHAPES = [(5000, 4001), (16385,), (7,), (3, 65537), (14345679,), (0,),
+              (1,)]
+    TYPES = [F32, BF, FH, F32, F32, F32, BF]
+
+    @pytest.mark.parametrize('max_norm', [0.3, 1e9])
+    def test_new_and_in_place(self, max_norm):
+        g = torch.Generator(device='cuda').manual_seed(11)
+        grads = [torch.randn(s, generator=g, device='cuda').to(t)
+                 for s, t in zip(self.SHAPES, self.TYPES)]
+        assert sum(t.numel() * t.element_size() for t in grads) >= 128 << 20
+        want, norm = _exact(grads, max_norm)
+        before = [t.clone() for t in grads]
+        new, n = gc.clip_grads(grads, max_norm)
+        _check(new, want, grads)
+        _check_norm(n, norm)
+        assert all(torch.equal(a, b) for a, b in zip(grads, before))
+        params = [torch.nn.Parameter(torch.empty_like(t)) for t in grads]
+        for p, t in zip(params, grads):
+            p.grad = t
+        _check_norm(gc.clip_grad_norm_(params, max_norm), norm)
+        assert all(torch.equal(a, b) for a, b in zip(grads, new))
+
+    @pytest.mark.parametrize('momentum,nesterov', [(0.0, False),
+                                                   (0.9, True)])
+    @pytest.mark.parametrize('max_norm', [0.25, 1e9])
+    def test_update(self, momentum, nesterov, max_norm):
+        g = torch.Generator(device='cuda').manual_seed(12)
+        shapes = self.SHAPES
+
+        def new():
+            return [torch.randn(s, generator=g, device='cuda')
+                    for s in shapes]
+        params, grads = new(), new()
+        moms = new() if momentum else []
+        wd, lr = 1e-2, 0.3
+        norm = sum(float(t.double().square().sum()) for t in grads) ** 0.5
+        f = min(1.0, max_norm / (norm + 1e-6))
+        old_p = [t.clone() for t in params]
+        old_m = [t.clone() for t in moms]
+        sgd = K.FusedSGD(params, grads, moms, [wd] * len(shapes),
+                         momentum=momentum, nesterov=nesterov)
+        assert sgd._past
+        got = sgd.step(lr, max_norm=max_norm)
+        assert abs(float(got) - norm) <= 1.01 * HALF * norm
+        for i, p in enumerate(params):   # as in TestClippedStep
+            q, d = old_p[i].double(), grads[i].double() * f
+            size = d.abs() + (wd * q).abs()
+            d = d + wd * q
+            if momentum:
+                b = momentum * old_m[i].double()
+                m = b + d
+                size = 2 * (size + b.abs())
+                d = d + momentum * m if nesterov else m
+                assert bool(((moms[i].double() - m).abs()
+                             <= 8 * HALF * size).all())
+            most = q.abs() + lr * size
+            assert bool(((p.double() - (q - lr * d)).abs()
+                         <= 8 * HALF * most).all())

@@ -724,3 +724,36 @@ def test_functions_refuse_to_be_traced():
                  lambda x, t: tl.token_log_probs(x, t).log_probs):
         with pytest.raises(RuntimeError):
             torch.jit.trace(call, (x, t))
+
+
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('rows,vocab', [(512, 3), (512, 17), (512, 256),
+                                        (700, 2500), (700, 10000),
+                                        (256, 32771), (64, 50001)])
+def test_to_a_few_roundings(rows, vocab, kind):
+    """Ordinary rows, closer than REL. An element passes at most the adds of
+    its thread's 65 elements and 24 more in the merges, 2 u for its own
+    exponential, and 2 u of its distance from the maximum, 2 M in the mean:
+    s is within (min(vocab, 65) + 28 + 3 M) u. A log probability and an
+    entropy add the roundings of 6 u of their size. That is the worst: errors
+    of both signs add up like the root of their number, 10 u for 89 of them,
+    and what always has the same sign, of log2 e and of the exponential, is
+    2 u + M u / 4, so over all rows the root mean square is held to half of
+    that worst or less."""
+    x, t = _make(rows, vocab, kind, seed=50, scale=2.0)
+    x.requires_grad_(True)
+    log, p, h = _exact(x)
+    best = log.amax(1, keepdim=True)
+    m = -(p * (log - best)).sum(1).detach()
+    lp = log.gather(1, t[:, None])[:, 0].detach()
+    h = h.detach()
+    adds = min(vocab, 65) + 28
+    r = tl.token_log_probs(x.detach(), t)
+    each = tl.cross_entropy(x.detach(), t, reduction='none')
+    for got, want, terms in ((r.log_probs, lp, 0.0), (each, -lp, 0.0),
+                             (r.entropy, h, m * adds)):
+        off = (got.double() - want).abs()
+        worst = (adds + 3 * m + 6 * want.abs() + terms) * U
+        assert bool((off <= worst).all()), float((off / worst).max())
+        mean = (12 + adds ** 0.5 + m + 3 * want.abs() + terms / 4) * U
+        assert float((off / mean).square().mean()) <= 1.0
