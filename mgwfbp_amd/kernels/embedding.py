@@ -4,9 +4,9 @@ gfx950 HIP kernels (embedding_kernels.hip).
 ``embedding`` looks rows of a table up by token and scales them;
 ``MgxEmbedding`` is nn.Embedding on it (the reference's word-level model,
 models/lstm.py:17). torch's gradient on a GPU sorts through a library and
-takes many launches; this one takes three for up to 16384 tokens, adds each
-token's rows up in the order of their positions, in float32, and rounds
-once, so a repeated call gives the same bits.
+takes many launches; this one takes three at most for up to 16384 tokens,
+adds each token's rows up in float32, in an order that the positions decide,
+and rounds once, so a repeated call gives the same bits.
 
 The weight is float32, bfloat16 or float16; its gradient is dense and of
 its type. A token outside the table is an IndexError on the CPU; on a GPU,

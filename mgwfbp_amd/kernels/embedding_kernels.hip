@@ -8,9 +8,11 @@
 // gradient reads N rows and writes V; adding rows to dW as they come would
 // take atomics, whose order changes the sums from run to run, so the
 // tokens are sorted first, stably, and each run of one token is added up
-// in the order of its positions, in 32 bits, and rounded once.
+// in 32 bits, in an order that its positions alone decide (one after the
+// other, or by parts where it is long), and rounded once.
 //
-// Up to 1024 tokens, owned_rows_kernel does all of it in one launch. More:
+// Up to 1024 tokens, owned_rows_kernel does all of it in one launch, unless
+// they are more than two for each row of the table. Otherwise:
 //
 //   1. sort. Up to 16384 tokens one block sorts them in LDS (a stable
 //      radix sort, at most 8 bits a pass), while the launch's other blocks
@@ -789,8 +791,8 @@ torch::Tensor weight_grad(const torch::Tensor& tokens,
 #define SORT(I, IPT)                                                      \
   launch_sort<I, IPT>(tokens, vocab, padding, pos_bits, key_bits, keys,   \
                       positions, grad)
-    if (n <= 1024) {
-      if (narrow) SORT(uint32_t, 1); else SORT(uint64_t, 1);
+    if (n <= 1024) {                  // and more than two for each row of dW
+      SORT(uint32_t, 1);
     } else if (n <= 4096) {
       if (narrow) SORT(uint32_t, 4); else SORT(uint64_t, 4);
     } else {

@@ -45,13 +45,6 @@ __device__ __forceinline__ u32x4 load16_past(const void* p) {
 __device__ __forceinline__ void store16_past(void* p, u32x4 v) {
   __builtin_nontemporal_store(v, static_cast<u32x4_any*>(p));
 }
-// `past`: the same for a whole launch.
-__device__ __forceinline__ u32x4 load16(const void* p, bool past) {
-  return past ? load16_past(p) : load16(p);
-}
-__device__ __forceinline__ void store16(void* p, u32x4 v, bool past) {
-  if (past) store16_past(p, v); else store16(p, v);
-}
 
 // One element type: how many sit in 16 bytes, and both conversions. Only
 // the rounding to the 16-bit types loses anything: half a step, to even.

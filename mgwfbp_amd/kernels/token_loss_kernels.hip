@@ -1051,7 +1051,7 @@ constexpr long kHeldFew = 8192;
 constexpr long kHeldLeast = 16;   // elements: a whole vector for certain
 
 template <typename F>
-bool with_slice(long vecs, bool few, F&& f) {
+bool with_shared(long vecs, F&& f) {
   using std::integral_constant;
   if (vecs <= 256)
     f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
@@ -1063,10 +1063,17 @@ bool with_slice(long vecs, bool few, F&& f) {
     f(integral_constant<int, 512>{}, integral_constant<int, 5>{});
   else if (vecs <= kHeldSlice)
     f(integral_constant<int, 512>{}, integral_constant<int, 8>{});
-  else if (few && vecs <= kHeldFew)
-    f(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
   else
     return false;
+  return true;
+}
+
+template <typename F>
+bool with_slice(long vecs, bool few, F&& f) {
+  using std::integral_constant;
+  if (with_shared(vecs, f)) return true;
+  if (!few || vecs > kHeldFew) return false;
+  f(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
   return true;
 }
 
@@ -1074,7 +1081,7 @@ bool with_slice(long vecs, bool few, F&& f) {
 template <typename F>
 bool with_row(long vecs, F&& f) {
   using std::integral_constant;
-  if (vecs <= kHeldSlice) return with_slice(vecs, false, f);
+  if (with_shared(vecs, f)) return true;
   if (vecs <= 9216)
     f(integral_constant<int, 768>{}, integral_constant<int, 12>{});
   else if (vecs <= 16384)

@@ -440,3 +440,12 @@ def test_function_refuses_to_be_traced():
     w, t = _weight(9, 4, F32), torch.tensor([1, 2], device='cuda')
     with pytest.raises(RuntimeError):
         torch.jit.trace(lambda t: em.embedding(t, w), (t,))
+
+
+@pytest.mark.parametrize('n,vocab', [
+    (1024, 511), (1024, 512), (1000, 40),       # sorted, and not, in one block
+    (2000, (1 << 21) + 5), (4096, 1 << 20),     # words of 64 bits, four each
+    (4097, (1 << 19) - 1), (1025, 1 << 31 >> 9)])
+@pytest.mark.parametrize('how', ['even', 'text', 'same'])
+def test_at_the_sorts_borders(n, vocab, how):
+    _both(_tokens(n, vocab, how), _weight(vocab, 3, BF), 1.0)
