@@ -419,6 +419,10 @@ __global__ __launch_bounds__(kBlock) void l2norm_sq_kernel(
   }
 }
 
+// A kernel, since a clip may be captured: hipMemsetAsync nodes have given
+// wrong results on replays after the first.
+__global__ void clear_kernel(float* __restrict__ x) { *x = 0.f; }
+
 // Squared-L2 of a flat fp32 buffer (grid-stride, wave64 shuffle reduce,
 // one atomicAdd per block). Feeds clip_scale_kernel: together they form
 // the device-side gradient clip (reference distributed_optimizer.py:
@@ -722,8 +726,8 @@ void l2norm_clip_(torch::Tensor buf, torch::Tensor normsq_scratch,
   auto stream = c10::hip::getCurrentHIPStream().stream();
   const int grid = std::max(
       1L, std::min((long)kMaxGrid, (n + kBlock * 4 - 1) / (kBlock * 4)));
-  CHECK_HIP(hipMemsetAsync(normsq_scratch.data_ptr(), 0, sizeof(float),
-                           stream));
+  hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1), 0, stream,
+                     normsq_scratch.data_ptr<float>());
   hipLaunchKernelGGL(l2norm_sq_flat_kernel, dim3(grid), dim3(kBlock), 0,
                      stream, buf.data_ptr<float>(), n,
                      normsq_scratch.data_ptr<float>());

@@ -392,3 +392,29 @@ class TestPastTheCache:
             most = q.abs() + lr * size
             assert bool(((p.double() - (q - lr * d)).abs()
                          <= 8 * HALF * most).all())
+
+
+def test_flat_clip_captured():
+    """The clip of one merged buffer, replayed between eager calls. Its sum
+    of squares is in float32 and in any order: n u at the worst, of which the
+    root halves, beside a few roundings."""
+    n = 70001
+    buf = torch.zeros(n, device='cuda')
+    src = _grads([(n,)], [F32], seed=7)[0]
+    buf.copy_(src)
+    K.l2norm_clip_(buf, 0.5)             # makes its scratch
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        K.l2norm_clip_(buf, 0.5)
+    for k in range(5):
+        buf.copy_(src * (k + 1))
+        want = src.double() * (k + 1)
+        want *= min(1.0, 0.5 / (float(want.square().sum()) ** 0.5 + 1e-6))
+        g.replay()
+        torch.cuda.synchronize()
+        far = (n / 2 + 8) * HALF
+        assert bool(((buf.double() - want).abs() <= far * want.abs()).all())
+        other = src * (k + 2)
+        K.l2norm_clip_(other, 0.5)
+        assert abs(float(other.double().norm()) - 0.5) <= far * 0.5 + 1e-6
