@@ -418,3 +418,27 @@ def test_flat_clip_captured():
         other = src * (k + 2)
         K.l2norm_clip_(other, 0.5)
         assert abs(float(other.double().norm()) - 0.5) <= far * 0.5 + 1e-6
+
+
+def test_flat_clips_at_once():
+    """Two captured clips replayed on two streams at once: each has its own
+    sum of squares, of which one is 10^4 times the other."""
+    n = 1 << 20
+    src = [torch.full((n,), s, device='cuda') for s in (0.01, 1.0)]
+    bufs = [s.clone() for s in src]
+    graphs = [torch.cuda.CUDAGraph() for _ in src]
+    torch.cuda.synchronize()
+    for buf, graph in zip(bufs, graphs):
+        with torch.cuda.graph(graph):
+            buf.copy_(src[0] if buf is bufs[0] else src[1])
+            K.l2norm_clip_(buf, 0.5)
+    streams = [torch.cuda.Stream() for _ in src]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for buf in bufs:                 # all elements are 0.5 / 2^10
+            assert torch.allclose(buf, torch.full_like(buf, 0.5 / 1024),
+                                  rtol=1e-3, atol=0)
