@@ -31,7 +31,7 @@
 // done again by slow_row, which subtracts first and takes every case; its
 // stats are told apart by a negative s.
 //
-// Measured: 8190 x 50001 bf16, loss and gradient 304 us, of which 296 (5.5
+// Measured: 8190 x 50001 bf16, loss and gradient 304 us, of which 299 (5.5
 // TB/s) in row_loss_kernel; 4095 x 32768 bf16, log probabilities with
 // entropy 52 us (5.1 TB/s) and their gradient 87 (6.1 TB/s); 700 x 10000
 // float32 with the best five 10 us; 4 x 50001 bf16 with the best eight 10.

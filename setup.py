@@ -23,8 +23,9 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 
 # Device code is built without packed fp32 arithmetic: hipcc -O3 forms
 # v_pk_{add,mul,fma}_f32 from ordinary float code by itself, and some of
-# their forms have given wrong results on gfx950. The kernels here are
-# bound by memory, so the scalar forms cost nothing. (hipcc's host pass
+# their forms have given wrong results on gfx950. Nearly all kernels here
+# are bound by memory; what the scalar forms cost beside the packed ones has
+# not been measured, as the packed ones are not run. (hipcc's host pass
 # warns that it does not know the feature; that is harmless.)
 common_args = {
     'cxx': ['-O3', '-std=c++17'],
