@@ -102,12 +102,13 @@ class MgxCrossEntropyLoss(nn.CrossEntropyLoss):
         return (x.is_cuda and x.dtype in _TYPES and x.dim() == 2
                 and y.dim() == 1 and y.dtype in (torch.int64, torch.int32)
                 and x.size(0) == y.size(0) and self.weight is None
+                and self.reduction in _REDUCTIONS
                 and self.label_smoothing == 0.0 and seen_whole(x, y))
 
     def forward(self, x, y):
         if not self._use_hip_path(x, y):
             return super().forward(x, y)
-        return load_lm().cross_entropy(x, y, self.ignore_index,
+        return load_lm().cross_entropy(x, y, int(self.ignore_index),
                                        _REDUCTIONS[self.reduction], False,
                                        True)
 

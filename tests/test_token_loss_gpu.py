@@ -757,3 +757,11 @@ def test_to_a_few_roundings(rows, vocab, kind):
         assert bool((off <= worst).all()), float((off / worst).max())
         mean = (12 + adds ** 0.5 + m + 3 * want.abs() + terms / 4) * U
         assert float((off / mean).square().mean()) <= 1.0
+
+
+def test_module_refuses_an_unknown_reduction():
+    x, t = _make(3, 20, torch.float32)
+    loss = tl.MgxCrossEntropyLoss()
+    loss.reduction = 'max'
+    with pytest.raises(ValueError):
+        loss(x, t)
