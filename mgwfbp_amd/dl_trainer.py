@@ -583,6 +583,7 @@ class DLTrainer:
                         continue
                     out, _ = self.net(x, hidden)
                     score = (token_log_probs if settings.USE_HIP_KERNELS
+                             and out.dtype != torch.float64
                              else token_log_probs_reference)
                     r = score(out, y, top_k=min(5, self.net.ntokens),
                               ignore_index=self.criterion.ignore_index)

@@ -235,3 +235,21 @@ def test_evaluation_leaves_ignored_targets_out():
     t = _word_level(batches)
     assert math.log(t.test(0)) == pytest.approx(sum(want) / 3, rel=1e-6)
     assert t.top5_accuracy == pytest.approx(sum(hits) / 3, abs=1e-12)
+
+
+def test_evaluation_of_a_model_in_64_bits(monkeypatch):
+    """The kernels take no float64 logits; such a model is scored by the
+    plain form, wherever it lies."""
+    from mgwfbp_amd import dl_trainer
+
+    def kernels(logits, targets, **kw):
+        raise TypeError('logits must be float32, bfloat16 or float16')
+
+    monkeypatch.setattr(dl_trainer, 'token_log_probs', kernels)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(4, 5, 40, generator=g, dtype=torch.float64)
+    y = torch.randint(0, 40, (4, 5), generator=g)
+    ppl = _word_level([(x, y)]).test(0)
+    assert math.log(ppl) == pytest.approx(float(
+        torch.nn.functional.cross_entropy(x.view(-1, 40), y.view(-1))),
+        rel=1e-12)
